@@ -364,6 +364,82 @@ int skinny_qmm_w4g64_noalloc(const void* x, int ldx, const void* w_tc, void* out
  * allocates nothing. */
 int skinny_qmm_w4g64_noalloc_errors(void* dst, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged key-value caches of a batch of sequences.
+ *
+ * A pool holds n_pages pages; a page holds `page` consecutive positions of one sequence, element
+ * [page id][kv head][slot][dim] (dense inside a page; pages k_page_stride / v_page_stride elements
+ * apart, a multiple of D; 16-byte aligned).  Sequence b's position j is in slot j % page of page
+ * table[b * table_stride + j / page] (int32, width entries per sequence; page * width < 2^31).
+ * kv_type 0: bf16 pages; 1: e4m3 pages with one f32 scale per kv head (value = stored * scale).
+ * D is 64, 128 or 256.
+ *
+ * lengths [B] int32 (device): the tokens in the cache BEFORE the step; counts [B] int32 (device, may
+ * be NULL): the step's new tokens of each sequence, 0 .. T (NULL: T each).  New token t sits at
+ * position lengths[b] + t.  Rows t >= counts[b] are padding: nothing is appended for them and their
+ * outputs are zero, so a batch can have idle slots.  After the step the caller adds the counts.
+ * q_strides, k_strides, v_strides are HOST arrays of 3 element strides (batch, token, head),
+ * multiples of 8; dims are dense and rows 16-byte aligned.
+ *
+ * What the kernels read from the device is checked there: a sequence with lengths < 0, counts
+ * outside [0, T] or lengths + counts > page * width takes no part (its outputs are zero); a page id
+ * outside [0, n_pages) is skipped (nothing is written, its keys are not seen).  Both set bit 9 of the
+ * device's paged error word (skinny_paged_errors).  No counterpart in the reference (one sequence,
+ * contiguous caches).
+ * ------------------------------------------------------------------------------------------- */
+
+/* Append a step's keys and values (k, v bf16 [B, T, Hkv, D]) to the pages, rotating queries
+ * (q bf16 [B, T, Hq, D], may be NULL; rotated into q_out, dense) and keys on the way:
+ * rotate-half on the first rot dims (rot % 16 == 0, 0 <= rot <= D) by position * inv_freq[j]
+ * (f32 [rot / 2]; the angle is formed in f64).  e4m3 pages take x / scale rounded to nearest and
+ * saturated to +-448.  A page that is written belongs to one sequence.  q_out must not overlap q.
+ * One launch (programmatic dependent launch). */
+int skinny_paged_append(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                        const void* v, const long long* v_strides, void* q_out, void* k_pages, void* v_pages,
+                        long long k_page_stride, long long v_page_stride, int kv_type, const float* k_scale,
+                        const float* v_scale, const int32_t* table, long long table_stride, int width, int n_pages,
+                        int page, const int32_t* lengths, const int32_t* counts, const float* inv_freq, int rot, int B,
+                        int T, int Hq, int Hkv, int D, void* stream);
+
+/* Workspace bytes of skinny_paged_attn (0 when the shape is not supported).  It holds partial
+ * results between the call's launches and no state between calls; it needs no initialisation. */
+size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D);
+
+/* Attention of the step's T <= 16 new tokens per sequence (already appended) over its pages:
+ * out[b, t, h] (bf16, dense [B, T, Hq, D]) = softmax(scale * q . k_j) v over the positions
+ * j <= lengths[b] + t, and j > lengths[b] + t - window when window > 0; query head h reads kv head
+ * h / (Hq / Hkv).  lse (f32 [B, T, Hq], may be NULL) = ln sum_j exp(scale * q . k_j).  A row that
+ * sees no key has output 0 and lse -inf.  Keys a row does not see have no influence on it, whatever
+ * they hold (infinities and NaN included). */
+int skinny_paged_attn(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
+                      long long k_page_stride, long long v_page_stride, int kv_type, const float* k_scale,
+                      const float* v_scale, const int32_t* table, long long table_stride, int width, int n_pages,
+                      int page, const int32_t* lengths, const int32_t* counts, float scale, int window, void* out,
+                      float* lse, int B, int T, int Hq, int Hkv, int D, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* The current device's paged error word (0: none; sticky), copied as one uint32 to dst (may be NULL)
+ * in stream order, then cleared when clear != 0. */
+int skinny_paged_errors(void* dst, int clear, void* stream);
+
+/* Workspace bytes of skinny_token_logprobs (0 when the shape is not supported); scratch of one call,
+ * needs no initialisation. */
+size_t skinny_token_logprobs_workspace_bytes(int rows, int V, int top);
+
+/* Log probabilities under rows of logits x [rows, V] (type 0: bf16, 1: f32; row stride ld, rows need
+ * only their element's alignment):
+ *   logprobs[r] = x[r, tokens[r]] - lse_r, lse_r = ln sum_v exp x[r, v]; -inf for a token outside
+ *                 [0, V) (e.g. -1: none)
+ *   entropy[r]  = -sum p ln p  (nats)
+ *   top_ids, top_logprobs [rows, top]: the top <= 32 most likely tokens, by value, ties to the
+ *                 lowest index, a NaN above every number (the order of skinny_spec_accept)
+ * A logit of -inf has probability 0; a row of nothing else has logprobs -inf and entropy 0; a row
+ * that holds a NaN or +inf has NaN logprobs (of tokens in range) and entropy.  Sums are held in f32.
+ * The scoring counterpart of the argmax in skinny_spec_accept. */
+int skinny_token_logprobs(const void* logits, long long ld, int type, int rows, int V, const int32_t* tokens, int top,
+                          float* logprobs, float* entropy, float* top_logprobs, int32_t* top_ids, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,7 +6,7 @@ There is no fallback: if `_skinny_b200.so` is missing or does not load, every op
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_int, c_size_t, c_uint32, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "_skinny_b200.so"
@@ -79,6 +79,17 @@ SIGNATURES = {
                                          c_void_p, c_int, c_int, c_int, c_void_p]),
     "skinny_qmm_w4g64_swiglu": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t,
                                         c_void_p]),
+    "skinny_paged_append": (c_int, [c_void_p] * 9 + [c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p] + [c_int] * 6
+                            + [c_void_p]),
+    "skinny_paged_attn_workspace_bytes": (c_size_t, [c_int] * 5),
+    "skinny_paged_attn": (c_int, [c_void_p] * 4 + [c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_longlong,
+                                  c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_int, c_void_p, c_void_p]
+                          + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "skinny_paged_errors": (c_int, [c_void_p, c_int, c_void_p]),
+    "skinny_token_logprobs_workspace_bytes": (c_size_t, [c_int] * 3),
+    "skinny_token_logprobs": (c_int, [c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int] + [c_void_p] * 5
+                              + [c_size_t, c_void_p]),
 }
 
 

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 
 #include "../../include/skinny_b200.h"
+#include "logprobs.cuh"
+#include "paged.cuh"
 #include "qmm_layout.cuh"
 
 namespace skinny {
@@ -564,6 +566,156 @@ int skinny_gdn_rollback_tree(int n_layers, float* const* state, const float* con
   }
   return cuda_status(skinny::gdn_rollback_tree_call(n_layers, state, ckpt, conv, conv_full, state_elems, node, rows,
                                                     W, C, static_cast<cudaStream_t>(stream)));
+}
+
+// ---- paged caches ----
+static int paged_seqs(skinny::PagedSeqs& s, const int32_t* table, long long table_stride, int width, int n_pages,
+                      int page, const int32_t* lengths, const int32_t* counts, int B, int T) {
+  if (!table || !lengths) return SKINNY_ERR_INVALID_ARG;
+  if (B < 1 || B > skinny::kPagedMaxBatch || T < 1 || static_cast<long long>(B) * T > INT32_MAX) return SKINNY_ERR_SHAPE;
+  if (page < 1 || n_pages < 1 || width < 1 || static_cast<long long>(width) * page > INT32_MAX) return SKINNY_ERR_SHAPE;
+  if (table_stride < width && B > 1) return SKINNY_ERR_INVALID_ARG;
+  if (!aligned4(table) || !aligned4(lengths) || !aligned4(counts)) return SKINNY_ERR_ALIGNMENT;
+  s = skinny::PagedSeqs{lengths, counts, table, table_stride, width, page, n_pages, B, T, nullptr};
+  return SKINNY_OK;
+}
+
+// Pages of a pool: aligned, dense inside a page, the scales of an 8-bit pool.
+static int check_pages(const void* p, long long stride, int kv_type, const float* scale, int Hkv, int page, int D) {
+  if (!p || kv_type < 0 || kv_type > 1 || (kv_type == 1 && !scale)) return SKINNY_ERR_INVALID_ARG;
+  if (Hkv < 1 || Hkv > 1024 || (D != 64 && D != 128 && D != 256)) return SKINNY_ERR_SHAPE;
+  if (stride < static_cast<long long>(Hkv) * page * D) return SKINNY_ERR_INVALID_ARG;
+  if (!aligned16(p) || stride % D || !aligned4(scale)) return SKINNY_ERR_ALIGNMENT;
+  return SKINNY_OK;
+}
+
+static int check_rows(const void* p, const long long* stride) {
+  if (!p || !stride) return SKINNY_ERR_INVALID_ARG;
+  if (!aligned16(p) || stride[0] % 8 || stride[1] % 8 || stride[2] % 8) return SKINNY_ERR_ALIGNMENT;
+  return SKINNY_OK;
+}
+
+int skinny_paged_append(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                        const void* v, const long long* v_strides, void* q_out, void* k_pages, void* v_pages,
+                        long long k_page_stride, long long v_page_stride, int kv_type, const float* k_scale,
+                        const float* v_scale, const int32_t* table, long long table_stride, int width, int n_pages,
+                        int page, const int32_t* lengths, const int32_t* counts, const float* inv_freq, int rot, int B,
+                        int T, int Hq, int Hkv, int D, void* stream) {
+  skinny::PagedAppendParams prm{};
+  int st = check_pages(k_pages, k_page_stride, kv_type, k_scale, Hkv, page, D);
+  if (st == SKINNY_OK) st = check_pages(v_pages, v_page_stride, kv_type, v_scale, Hkv, page, D);
+  if (st == SKINNY_OK) st = check_rows(k, k_strides);
+  if (st == SKINNY_OK) st = check_rows(v, v_strides);
+  if (st == SKINNY_OK && q) st = check_rows(q, q_strides);
+  if (st != SKINNY_OK) return st;
+  if ((q && !q_out) || (rot > 0 && !inv_freq)) return SKINNY_ERR_INVALID_ARG;
+  if (rot < 0 || rot > D || rot % 16 || (q && (Hq < 1 || Hq > 65536))) return SKINNY_ERR_SHAPE;
+  if (!aligned16(q_out) || !aligned4(inv_freq)) return SKINNY_ERR_ALIGNMENT;
+  st = paged_seqs(prm.seq, table, table_stride, width, n_pages, page, lengths, counts, B, T);
+  if (st != SKINNY_OK) return st;
+  prm.q = static_cast<const __nv_bfloat16*>(q);
+  prm.k = static_cast<const __nv_bfloat16*>(k);
+  prm.v = static_cast<const __nv_bfloat16*>(v);
+  for (int i = 0; i < 3; ++i) {
+    prm.qs[i] = q ? q_strides[i] : 0;
+    prm.ks[i] = k_strides[i];
+    prm.vs[i] = v_strides[i];
+  }
+  prm.q_out = static_cast<__nv_bfloat16*>(q_out);
+  prm.kp = k_pages;
+  prm.vp = v_pages;
+  prm.kps = k_page_stride;
+  prm.vps = v_page_stride;
+  prm.k_scale = k_scale;
+  prm.v_scale = v_scale;
+  prm.inv_freq = inv_freq;
+  prm.rot = rot;
+  prm.Hq = q ? Hq : 0;
+  prm.Hkv = Hkv;
+  prm.D = D;
+  const cudaError_t e = skinny::paged_error_word(current_device(), &prm.seq.err);
+  if (e != cudaSuccess) return cuda_status(e);
+  return cuda_status(skinny::paged_append_launch(prm, kv_type == 1, skinny::device_sm_count(current_device()),
+                                                 static_cast<cudaStream_t>(stream)));
+}
+
+size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D) {
+  if (B < 1 || B > skinny::kPagedMaxBatch || T < 1 || T > skinny::kPagedMaxTokens || Hkv < 1 || Hkv > 1024 || Hq < 1 ||
+      Hq % Hkv || (D != 64 && D != 128 && D != 256))
+    return 0;
+  return skinny::paged_attn_ws_bytes(B, T, Hq, Hkv, D, skinny::device_sm_count(current_device()));
+}
+
+int skinny_paged_attn(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
+                      long long k_page_stride, long long v_page_stride, int kv_type, const float* k_scale,
+                      const float* v_scale, const int32_t* table, long long table_stride, int width, int n_pages,
+                      int page, const int32_t* lengths, const int32_t* counts, float scale, int window, void* out,
+                      float* lse, int B, int T, int Hq, int Hkv, int D, void* workspace, size_t workspace_bytes,
+                      void* stream) {
+  skinny::PagedAttnParams prm{};
+  int st = check_pages(k_pages, k_page_stride, kv_type, k_scale, Hkv, page, D);
+  if (st == SKINNY_OK) st = check_pages(v_pages, v_page_stride, kv_type, v_scale, Hkv, page, D);
+  if (st == SKINNY_OK) st = check_rows(q, q_strides);
+  if (st != SKINNY_OK) return st;
+  if (!out || window < 0) return SKINNY_ERR_INVALID_ARG;
+  if (T < 1 || T > skinny::kPagedMaxTokens) return SKINNY_ERR_TOKENS;
+  if (Hq < 1 || Hq % Hkv || static_cast<long long>(B) * T * Hq > INT32_MAX) return SKINNY_ERR_SHAPE;
+  if (!aligned16(out) || !aligned4(lse)) return SKINNY_ERR_ALIGNMENT;
+  st = paged_seqs(prm.seq, table, table_stride, width, n_pages, page, lengths, counts, B, T);
+  if (st != SKINNY_OK) return st;
+  const size_t need = skinny_paged_attn_workspace_bytes(B, T, Hq, Hkv, D);
+  if (!workspace || need == 0 || workspace_bytes < need || !aligned16(workspace)) return SKINNY_ERR_WORKSPACE;
+  prm.q = static_cast<const __nv_bfloat16*>(q);
+  for (int i = 0; i < 3; ++i) prm.qs[i] = q_strides[i];
+  prm.kp = k_pages;
+  prm.vp = v_pages;
+  prm.kps = k_page_stride;
+  prm.vps = v_page_stride;
+  prm.k_scale = k_scale;
+  prm.v_scale = v_scale;
+  prm.scale = scale;
+  prm.window = window;
+  prm.Hq = Hq;
+  prm.Hkv = Hkv;
+  prm.D = D;
+  prm.out = static_cast<__nv_bfloat16*>(out);
+  prm.lse = lse;
+  const cudaError_t e = skinny::paged_error_word(current_device(), &prm.seq.err);
+  if (e != cudaSuccess) return cuda_status(e);
+  return cuda_status(skinny::paged_attn_launch(prm, kv_type == 1, workspace, skinny::device_sm_count(current_device()),
+                                               static_cast<cudaStream_t>(stream)));
+}
+
+int skinny_paged_errors(void* dst, int clear, void* stream) {
+  uint32_t* word = nullptr;
+  if (!dst && !clear) return SKINNY_ERR_INVALID_ARG;
+  cudaError_t e = skinny::paged_error_word(current_device(), &word);
+  if (e == cudaSuccess && dst)
+    e = cudaMemcpyAsync(dst, word, sizeof(uint32_t), cudaMemcpyDefault, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess && clear) e = cudaMemsetAsync(word, 0, sizeof(uint32_t), static_cast<cudaStream_t>(stream));
+  return cuda_status(e);
+}
+
+// ---- log probabilities ----
+size_t skinny_token_logprobs_workspace_bytes(int rows, int V, int top) {
+  if (rows < 1 || V < 1 || top < 0 || top > skinny::kLpMaxTop || top > V) return 0;
+  return skinny::logprob_ws_bytes(rows, V, top, skinny::device_sm_count(current_device()));
+}
+
+int skinny_token_logprobs(const void* logits, long long ld, int type, int rows, int V, const int32_t* tokens, int top,
+                          float* logprobs, float* entropy, float* top_logprobs, int32_t* top_ids, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  if (!logits || !tokens || !logprobs || !entropy || type < 0 || type > 1) return SKINNY_ERR_INVALID_ARG;
+  if (top > 0 && (!top_logprobs || !top_ids)) return SKINNY_ERR_INVALID_ARG;
+  const size_t need = skinny_token_logprobs_workspace_bytes(rows, V, top);
+  if (need == 0 || (rows > 1 && ld < V)) return SKINNY_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(logits) & (type ? 3u : 1u)) || !aligned4(tokens) || !aligned4(logprobs) ||
+      !aligned4(entropy) || !aligned4(top_logprobs) || !aligned4(top_ids))
+    return SKINNY_ERR_ALIGNMENT;
+  if (!workspace || workspace_bytes < need || !aligned16(workspace)) return SKINNY_ERR_WORKSPACE;
+  const skinny::LogprobParams prm{logits, ld, rows, V, top, tokens, logprobs, entropy, top_logprobs, top_ids};
+  return cuda_status(skinny::logprob_launch(prm, type == 1, workspace, skinny::device_sm_count(current_device()),
+                                            static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,511 @@
+"""Paged cache append and attention against the f64 oracle."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import paged as opaged
+
+F8 = torch.float8_e4m3fn
+
+
+def test_oracle_attention_is_a_softmax():
+    """One sequence, pages in order: the oracle equals torch's softmax over the causal scores."""
+    torch.manual_seed(0)
+    q, k, v = torch.randn(1, 3, 4, 64), torch.randn(5, 2, 4, 64), torch.randn(5, 2, 4, 64)
+    o, lse, spread, dots, bad = opaged.attention(q, k, v, torch.arange(5)[None].int(), [14], None)
+    kk, vv = (x.transpose(1, 2).reshape(20, 2, 64).double().repeat_interleave(2, 1) for x in (k, v))
+    for t in range(3):
+        s = torch.einsum("hd,jhd->hj", q[0, t].double(), kk[:15 + t]) / 8
+        assert torch.allclose(o[0, t], torch.einsum("hj,jhd->hd", s.softmax(-1), vv[:15 + t]))
+        assert torch.allclose(lse[0, t], s.logsumexp(-1))
+    assert not bad and (spread >= o.abs() - 1e-12).all() and (dots > 0).all()
+    # window 1: a token sees itself; idle slots and sequences out of range see nothing
+    o, lse, *_ = opaged.attention(q, k, v, torch.arange(5)[None].int(), [14], None, window=1)
+    assert torch.allclose(o[0, 1], vv[15])
+    assert opaged.attention(q, k, v, torch.arange(5)[None].int(), [14], [0])[1].eq(-math.inf).all()
+    assert opaged.attention(q, k, v, torch.arange(5)[None].int(), [18], None)[4]
+    assert opaged.attention(q, k, v, torch.tensor([[0, 1, 5, 3, 4]]).int(), [14], None)[4]
+
+
+# ---------------------------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------------------------
+F = 0x10000  # a pointer that is never touched
+
+
+def _strides(*s):
+    import ctypes
+
+    return (ctypes.c_longlong * 3)(*s)
+
+
+def _append_status(**kw):
+    from skinny_mlx_b200 import _lib
+
+    a = dict(q=F, qs=_strides(512, 512, 128), k=F, ks=_strides(256, 256, 128), v=F, vs=_strides(256, 256, 128), qo=F, kp=F,
+             vp=F, kps=2 * 16 * 128, vps=2 * 16 * 128, kv=0, ksc=None, vsc=None, table=F, ts=4, width=4, n=9, page=16,
+             lengths=F, counts=None, inv=F, rot=32, B=2, T=1, Hq=4, Hkv=2, D=128, stream=None)
+    a.update(kw)
+    return _lib.lib().skinny_paged_append(*a.values())
+
+
+def _attn_status(**kw):
+    from skinny_mlx_b200 import _lib
+
+    a = dict(q=F, qs=_strides(512, 512, 128), kp=F, vp=F, kps=2 * 16 * 128, vps=2 * 16 * 128, kv=0, ksc=None, vsc=None,
+             table=F, ts=4, width=4, n=9, page=16, lengths=F, counts=None, scale=0.1, window=0, out=F, lse=F, B=2, T=1, Hq=4,
+             Hkv=2, D=128, ws=F, wsn=1 << 40, stream=None)
+    a.update(kw)
+    return _lib.lib().skinny_paged_attn(*a.values())
+
+
+COMMON = [(dict(kp=None), -1), (dict(vp=None), -1), (dict(kv=2), -1), (dict(kv=1), -1), (dict(kv=1, ksc=F), -1),
+          (dict(Hkv=0), -2), (dict(D=96), -2), (dict(kps=2 * 16 * 128 - 128), -1), (dict(vps=2 * 16 * 128 + 8), -4),
+          (dict(kp=F + 8), -4), (dict(table=None), -1), (dict(lengths=None), -1), (dict(B=0), -2), (dict(B=8193), -2),
+          (dict(page=0, kps=1 << 20, vps=1 << 20), -2), (dict(n=0), -2), (dict(width=0), -2), (dict(width=1 << 27, ts=1 << 27), -2),
+          (dict(ts=3), -1), (dict(table=F + 2), -4), (dict(counts=F + 1), -4), (dict(q=F + 8), -4),
+          (dict(qs=_strides(512, 516, 128)), -4), (dict(qs=None), -1)]
+
+
+@pytest.mark.parametrize("kw,status", COMMON + [
+    (dict(k=None), -1), (dict(v=None), -1), (dict(qo=None), -1), (dict(inv=None), -1), (dict(rot=24), -2),
+    (dict(rot=144), -2), (dict(rot=-16), -2), (dict(Hq=0), -2), (dict(T=0), -2), (dict(T=1 << 30), -2), (dict(qo=F + 8), -4),
+    (dict(k=F + 2), -4), (dict(vs=_strides(256, 256, 100)), -4)])
+def test_append_entry_refuses(kw, status):
+    assert _append_status(**kw) == status
+
+
+@pytest.mark.parametrize("kw,status", COMMON + [
+    (dict(q=None), -1), (dict(out=None), -1), (dict(window=-1), -1), (dict(T=0), -3), (dict(T=17), -3), (dict(Hq=3), -2),
+    (dict(Hq=0), -2), (dict(out=F + 8), -4), (dict(lse=F + 2), -4), (dict(ws=None), -5), (dict(wsn=0), -5), (dict(ws=F + 4), -5)])
+def test_attention_entry_refuses(kw, status):
+    assert _attn_status(**kw) == status
+
+
+def test_workspace_of_unsupported_shapes_is_zero():
+    from skinny_mlx_b200 import _lib
+
+    ws = _lib.lib().skinny_paged_attn_workspace_bytes
+    for bad in ((0, 1, 4, 2, 128), (8193, 1, 4, 2, 128), (1, 17, 4, 2, 128), (1, 1, 4, 3, 128), (1, 1, 4, 2, 96), (1, 1, 0, 2, 64)):
+        assert ws(*bad) == 0
+
+
+def test_cpu_tensors_are_refused():
+    from skinny_mlx_b200 import paged
+
+    x, i = torch.zeros(2, 1, 2, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    pool = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.attention(x, pool, pool, i[:, None], i)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.append(x, x, x, pool, pool, i[:, None], i)
+
+
+# ---------------------------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------------------------
+class Case:
+    """A pool, a table of shuffled pages and a step's inputs on the device."""
+
+    def __init__(self, dev, lengths, counts=None, T=1, Hq=4, Hkv=2, D=128, page=16, kv=torch.bfloat16, seed=0, spare=3,
+                 gap=0, gated=False, width=None, std=1.0):
+        gen = torch.Generator().manual_seed(seed)
+        B = len(lengths)
+        self.B, self.T, self.Hq, self.Hkv, self.D, self.page, self.kv, self.dev = B, T, Hq, Hkv, D, page, kv, dev
+        self.width = width or max(1, max(-(-(n + T) // page) for n in lengths))
+        self.n_pages = B * self.width + spare
+        self.table = torch.randperm(self.n_pages, generator=gen)[:B * self.width].view(B, -1).int().to(dev)
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device=dev)
+        self.counts = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=dev)
+        per = 2 * D if gated else D
+        row = (torch.randn(B, T, Hq * per + 2 * Hkv * D, generator=gen) * std).bfloat16().to(dev)
+        self.q = row[..., :Hq * per].unflatten(-1, (Hq, per))[..., :D]
+        self.k = row[..., Hq * per:Hq * per + Hkv * D].unflatten(-1, (Hkv, D))
+        self.v = row[..., Hq * per + Hkv * D:].unflatten(-1, (Hkv, D))
+        pages = []
+        self.scales = {"k_scale": None, "v_scale": None}
+        for name in self.scales:
+            x = torch.randn(self.n_pages, Hkv * page * D + gap * D, generator=gen) * std
+            if kv == F8:
+                self.scales[name] = (0.01 + 0.03 * torch.rand(Hkv, generator=gen)).to(dev)
+                x = (x / 0.025).clamp(-448, 448)
+            x = x.to(kv).to(dev)
+            pages.append(x[:, :Hkv * page * D].unflatten(1, (Hkv, page, D)))
+        self.kp, self.vp = pages
+
+    def args(self):
+        return self.kp, self.vp, self.table, self.lengths
+
+    def attend(self, **kw):
+        from skinny_mlx_b200 import paged
+
+        return paged.attention(self.q, *self.args(), counts=self.counts, return_lse=True, **self.scales, **kw)
+
+    def oracle(self, **kw):
+        cpu = lambda x: None if x is None else x.cpu()
+        wide = lambda x: x.float().cpu() if x.dtype == F8 else x.cpu()
+        return opaged.attention(self.q.cpu(), wide(self.kp), wide(self.vp), self.table.cpu(), self.lengths.cpu(),
+                                cpu(self.counts), **{n: cpu(s) for n, s in self.scales.items()}, **kw)
+
+
+def check_attention(got, want, D):
+    """o: the result's rounding to bf16 (2^-8 of it), the probabilities' rounding to 16 bits (2^-8 of
+    sum p |v|), and the scores' error: a dot product of D terms in f32, accumulated by the tensor core with
+    truncation (2^-22 of sum |q k| per step of 16 terms and 2^-23 per join) is off by e = (D / 8 + 8) 2^-23 dots,
+    which changes each p by at most 4 e of itself; f32 sums of p and p v add 2^-16.  lse is off by e, its own
+    f32 rounding and the sum of the exponentials (2^-17)."""
+    o, lse, spread, dots, _ = want
+    go, gl = got[0].double().cpu(), got[1].double().cpu()
+    e = (D / 8 + 8) * 2.0 ** -23 * dots
+    seen = lse > -math.inf
+    assert torch.equal(gl > -math.inf, seen)
+    tol = 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.0 ** -16 + 4 * e[..., None]) * spread * (1 + 2.0 ** -8) + 1e-30
+    err = (go - o).abs()
+    assert (err <= tol).all(), f"o off by {float((err / tol).max()):.3f} of its tolerance"
+    assert (go[~seen] == 0).all()
+    err = (gl - lse).abs()[seen]
+    tol = (e + 2.0 ** -17 + 2.0 ** -22 * lse.abs())[seen]
+    assert (err <= tol).all(), f"lse off by {float((err / tol).max()):.3f} of its tolerance"
+
+
+# ---------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------
+def check_append(c: Case, inv, with_q=True):
+    from skinny_mlx_b200 import paged
+
+    before = [c.kp.clone(), c.vp.clone()]
+    got = paged.append(c.q if with_q else None, c.k, c.v, *c.args(), inv, counts=c.counts, **c.scales)
+    cpu = lambda x: None if x is None else x.cpu()
+    q, writes, bad = opaged.append(cpu(c.q), cpu(c.k), cpu(c.v), cpu(c.table), cpu(c.lengths), cpu(c.counts), cpu(inv), c.page,
+                                   c.n_pages, **{n: cpu(s) for n, s in c.scales.items()})
+    assert bool(paged.device_errors(c.dev, clear=True)) == bad
+    # a rotated pair x c - y s in f32: c and s off by at most 2^-22, three roundings: (|x| + |y|) 2^-20
+    h = 0 if inv is None else inv.numel()
+
+    def size(x):  # |x| + |its partner|
+        a = x.double().abs().cpu()
+        if h:
+            s = a[..., :h] + a[..., h:2 * h]
+            a = torch.cat([s, s, a[..., 2 * h:]], -1)
+        return a
+
+    if with_q:
+        assert got.shape == c.q.shape and got.is_contiguous()
+        err = (got.cpu().double() - q).abs()
+        assert (err <= 2.0 ** -8 * q.abs() + 2.0 ** -20 * size(c.q)).all()
+    else:
+        assert got is None
+    # e4m3: half a step is 2^-4 of the value, 2^-10 below the smallest normal number
+    half = 2.0 ** -8 if c.kv != F8 else 2.0 ** -4
+    least = 0 if c.kv != F8 else 2.0 ** -10
+    mask = torch.zeros(c.n_pages, c.page, dtype=torch.bool)
+    for pid, slot, kr, vr in writes:
+        mask[pid, slot] = True
+    pages = [x.float().cpu().double() for x in (c.kp, c.vp)]
+    ks = 1.0 if c.scales["k_scale"] is None else c.scales["k_scale"].cpu().double()[:, None]
+    big = float(size(c.k).max())
+    for pid, slot, kr, vr in writes:
+        for x, want, slack in ((pages[0][pid, :, slot], kr, 2.0 ** -20 * big / ks), (pages[1][pid, :, slot], vr, 0)):
+            if c.kv == F8:
+                want = want.clamp(-448, 448)
+            assert ((x - want).abs() <= half * want.abs() + least + slack).all()
+    for old, new in zip(before, (c.kp, c.vp)):  # nothing else was touched
+        same = (old.view(torch.uint8) == new.view(torch.uint8)) if c.kv == F8 else (old.view(torch.int16) == new.view(torch.int16))
+        assert same.cpu().all(-1).transpose(1, 2)[~mask].all()
+    return got
+
+
+def inv_freq(dev, rot, theta=1e6):
+    return theta ** (-torch.arange(rot // 2, device=dev, dtype=torch.float32) / (rot // 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("D,rot,Hq,Hkv,page,T", [(128, 32, 16, 4, 16, 1), (128, 128, 40, 8, 64, 3), (64, 64, 3, 1, 7, 5),
+                                                 (256, 16, 4, 2, 1, 2), (256, 256, 2, 2, 33, 20), (64, 0, 1, 1, 8, 1),
+                                                 (128, 96, 5, 5, 24, 130)])
+def test_append_values(cuda_lib, dev, kv, D, rot, Hq, Hkv, page, T):
+    c = Case(dev, [0, 5, 63, 200], T=T, Hq=Hq, Hkv=Hkv, D=D, page=page, kv=kv, seed=D + T)
+    check_append(c, inv_freq(dev, rot) if rot else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+def test_append_ragged_batch_with_idle_slots(cuda_lib, dev, kv):
+    c = Case(dev, [0, 17, 40, 8, 300], counts=[4, 0, 1, 3, 4], T=4, kv=kv, page=16, gated=True, gap=5)
+    check_append(c, inv_freq(dev, 32))
+    c = Case(dev, [3], counts=[0], T=2, kv=kv)
+    assert (check_append(c, inv_freq(dev, 32)) == 0).all()
+    check_append(Case(dev, [3, 9], T=2, kv=kv), inv_freq(dev, 64), with_q=False)
+
+
+@pytest.mark.gpu
+def test_append_far_positions(cuda_lib, dev):
+    """Positions whose angle an f32 product would not hold."""
+    c = Case(dev, [1_048_570, 131_071, 16_777_217], T=4, page=64, width=4)
+    c.table = torch.zeros(3, (16_777_300 // 64), dtype=torch.int32, device=dev)
+    for b, n in enumerate((1_048_570, 131_071, 16_777_217)):
+        c.table[b, n // 64:(n + 3) // 64 + 1] = torch.arange(3 * b, 3 * b + (n + 3) // 64 + 1 - n // 64, device=dev).int()
+    check_append(c, inv_freq(dev, 128, 1e4))
+
+
+@pytest.mark.gpu
+def test_append_e4m3_special_values(cuda_lib, dev):
+    from skinny_mlx_b200 import paged
+
+    c = Case(dev, [0], kv=F8, D=64, Hkv=1, Hq=1)
+    x = torch.zeros(64)
+    x[:12] = torch.tensor([448.0, 464.0, 465.0, 1e30, -1e30, math.inf, -math.inf, math.nan, 2.0 ** -9, 2.0 ** -10, 2.0 ** -11, -0.0])
+    c.k[0, 0, 0] = x.to(dev)
+    c.v[0, 0, 0] = x.to(dev)
+    one = torch.ones(1, device=dev)
+    paged.append(None, c.k, c.v, *c.args(), k_scale=one, v_scale=one)
+    want = x.bfloat16().float().clamp(-448, 448).to(F8)
+    pid = int(c.table[0, 0])
+    for pool in (c.kp, c.vp):
+        got = pool[pid, 0, 0].cpu()
+        assert torch.equal(got.view(torch.uint8) & 0x7F, want.view(torch.uint8) & 0x7F)
+        assert torch.equal(got.float()[:7], want.float()[:7])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+def test_what_is_out_of_range_touches_nothing(cuda_lib, dev, kv):
+    """Sequences that do not fit their table, bad counts, page ids outside the pool: reported, the rest of the
+    batch unharmed.  (Every index is checked in the kernels before it forms an address.)"""
+    from skinny_mlx_b200 import paged
+
+    paged.device_errors(dev, clear=True)
+    c = Case(dev, [30, 40, 2, 5, 20, 31], T=2, page=16, kv=kv, seed=5, width=3)
+    c.lengths = torch.tensor([30, -1, 2, 2**31 - 1, 20, 47], dtype=torch.int32, device=dev)
+    c.table[2, 0], c.table[4, 1] = -1, c.n_pages
+    check_append(c, inv_freq(dev, 32))
+    got = c.attend()
+    assert paged.device_errors(dev, clear=True) == 1 << 9
+    check_attention(got, c.oracle(), c.D)
+    c = Case(dev, [30, 40, 2], counts=[3, -1, 2], T=2, page=16, kv=kv, seed=6)
+    check_append(c, inv_freq(dev, 32))
+    got = c.attend()
+    assert paged.device_errors(dev, clear=True) == 1 << 9
+    check_attention(got, c.oracle(), c.D)
+    assert paged.device_errors(dev) == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,T,page", [(4, 4, 1, 16), (8, 2, 1, 64), (10, 2, 1, 24), (8, 1, 1, 1), (6, 2, 3, 7), (16, 1, 2, 48),
+                                           (4, 1, 8, 16), (8, 2, 16, 32), (5, 1, 13, 100), (17, 1, 1, 16), (40, 1, 4, 8)])
+def test_attention_values(cuda_lib, dev, Hq, Hkv, T, page, D, kv):
+    c = Case(dev, [0, 1, 15, 64, 131, 257], T=T, Hq=Hq, Hkv=Hkv, D=D, page=page, kv=kv, seed=Hq + T)
+    check_attention(c.attend(), c.oracle(), D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("window", [1, 2, 16, 17, 100])
+@pytest.mark.parametrize("T", [1, 5, 16])
+def test_attention_window(cuda_lib, dev, window, T, kv):
+    c = Case(dev, [0, 3, 95, 300], T=T, Hq=6, Hkv=2, page=16, kv=kv, seed=window)
+    check_attention(c.attend(window=window), c.oracle(window=window), c.D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+def test_attention_ragged_counts_scale_and_strides(cuda_lib, dev, kv):
+    c = Case(dev, [0, 17, 400, 8, 90, 0], counts=[4, 0, 1, 3, 4, 0], T=4, Hq=8, Hkv=4, kv=kv, gated=True, gap=7)
+    check_attention(c.attend(scale=0.3), c.oracle(scale=0.3), c.D)
+    check_attention(c.attend(scale=-0.05), c.oracle(scale=-0.05), c.D)
+    # queries whose rows are not aligned, or whose dims are not dense, are copied
+    want = c.attend()
+    raw = torch.empty(c.q.numel() + 4, dtype=torch.bfloat16, device=dev)
+    odd = raw[4:].view(c.q.shape)
+    for q in (odd.copy_(c.q), c.q.transpose(2, 3).contiguous().transpose(2, 3), c.q.transpose(0, 1).contiguous().transpose(0, 1)):
+        c.q = q
+        assert all(torch.equal(a, b) for a, b in zip(c.attend(), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("lengths,page,T,Hq,Hkv", [([4096], 64, 1, 16, 4), ([2047], 16, 8, 16, 4), ([9001, 1], 32, 1, 8, 2),
+                                                   ([700 + 37 * i for i in range(40)], 16, 1, 8, 2), ([20011], 128, 1, 4, 1),
+                                                   ([63 * i for i in range(70)], 16, 2, 2, 2)])
+def test_attention_long_and_many(cuda_lib, dev, lengths, page, T, Hq, Hkv, kv):
+    c = Case(dev, lengths, T=T, Hq=Hq, Hkv=Hkv, page=page, kv=kv, seed=len(lengths))
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+def test_attention_sharp_and_large_scores(cuda_lib, dev):
+    """Scores far apart (one key takes everything, late or early) and large ones of both signs."""
+    c = Case(dev, [200, 333], T=2, Hq=8, Hkv=2, std=6.0, seed=2)
+    check_attention(c.attend(), c.oracle(), c.D)
+    for at in (0, 100, 198):
+        c = Case(dev, [199], T=1, Hq=4, Hkv=1, seed=at)
+        c.kp[int(c.table[0, at // 16]), 0, at % 16] = (c.q[0, 0, 1] * 9)
+        check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("T,window", [(1, None), (5, None), (5, 20), (16, None)])
+def test_what_is_not_seen_has_no_influence(cuda_lib, dev, T, window, kv):
+    """NaN and infinities behind the last position, before the window, in pages of nobody, and in later tokens of
+    the same draft leave the rows that do not see them as they were."""
+    c = Case(dev, [45, 130, 7], T=T, Hq=6, Hkv=2, page=16, kv=kv, seed=T)
+    want = c.attend(window=window)
+    bad = [math.nan] if kv == F8 else [math.nan, math.inf, -math.inf]
+    seen = torch.zeros(c.n_pages, 16, dtype=torch.bool)
+    for b, n in enumerate((45, 130, 7)):
+        for j in range(max(0, n + 1 - window) if window else 0, n + T):
+            seen[int(c.table[b, j // 16]), j % 16] = True
+    for x in bad:
+        for pool in (c.kp, c.vp):
+            pool.transpose(1, 2)[(~seen).to(dev)] = torch.tensor(x, device=dev).to(kv)
+        got = c.attend(window=window)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for t in range(1, T):  # token t's own key and value: rows before it do not change
+        for pool, x in ((c.kp, bad[0]), (c.vp, bad[-1])):
+            for b, n in enumerate((45, 130, 7)):
+                pool[int(c.table[b, (n + t) // 16]), :, (n + t) % 16] = torch.tensor(x, device=dev).to(kv)
+        got = c.attend(window=window)
+        # (two roundings of the result, 2^-7 of it, and of the probabilities, 2^-7 sum p |v|)
+        assert all(torch.allclose(a[:, :t].float(), b[:, :t].float(), rtol=2.0 ** -7, atol=2.0 ** -7) for a, b in zip(got, want))
+        assert got[0][:, t].isnan().all()
+        c = Case(dev, [45, 130, 7], T=T, Hq=6, Hkv=2, page=16, kv=kv, seed=T)
+
+
+@pytest.mark.gpu
+def test_infinite_values_that_are_seen(cuda_lib, dev):
+    """An infinite value reaches exactly the dims and the rows that see it."""
+    c = Case(dev, [30], T=6, Hq=4, Hkv=2, seed=4)
+    pid, slot = int(c.table[0, 33 // 16]), 33 % 16
+    c.vp[pid, 1, slot, 5] = math.inf
+    o = c.attend()[0].float()
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[0, 3:, 2:, 5] = True
+    assert torch.equal(o.isinf(), hit) and not o.isnan().any()
+
+
+@pytest.mark.gpu
+def test_shared_pages_and_one_page_twice(cuda_lib, dev):
+    """Sequences that share a prefix's pages, and a table that names a page twice."""
+    c = Case(dev, [70, 90, 64], T=1, Hq=4, Hkv=2, page=16, seed=8)
+    c.table[1, :4] = c.table[0, :4]
+    c.table[2, 1] = c.table[2, 0]
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda_lib, dev):
+    """Pages further than 2^32 bytes into a pool, and page strides that pass 2^31 elements in all."""
+    torch.manual_seed(0)
+    big = torch.empty(5, 1 << 30, dtype=torch.bfloat16, device=dev)  # 10 GB: page 4 starts 2^33 bytes in
+    c = Case(dev, [40], T=2, Hq=4, Hkv=2, page=16)
+    n = 2 * 16 * 128
+    for i, pool in enumerate(("kp", "vp")):
+        x = big[:, i * n:(i + 1) * n].unflatten(1, (2, 16, 128))
+        x.copy_(torch.randn(5, 2, 16, 128, device=dev))
+        setattr(c, pool, x)
+    c.n_pages = 5
+    c.table = torch.tensor([[4, 0, 3]], dtype=torch.int32, device=dev)
+    check_append(c, inv_freq(dev, 32))
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+def test_step_of_a_batch_streams_and_graphs(cuda_lib, dev):
+    """append then attention for several steps, eagerly, on another stream, and replayed from two graphs that
+    run side by side: the same bits, and the oracle's values."""
+    from skinny_mlx_b200 import paged
+
+    inv = inv_freq(dev, 32)
+
+    def steps(c, n=3):
+        outs = []
+        for _ in range(n):
+            q = paged.append(c.q, c.k, c.v, *c.args(), inv, counts=c.counts, **c.scales)
+            outs.append(paged.attention(q, *c.args(), counts=c.counts, return_lse=True, **c.scales))
+            c.lengths += c.counts
+        return outs
+
+    def case(i):
+        return Case(dev, [100 + i, 900, 0, 37], counts=[2, 1, 2, 0], T=2, Hq=8, Hkv=2, page=16, seed=i, width=64)
+
+    want, finals = [], []
+    for i in range(2):
+        c = case(i)
+        want.append(steps(c))
+        finals.append(c)
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    other = []
+    for i, s in enumerate(streams):
+        c = case(i)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            other.append(steps(c))
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        c = case(i)
+        torch.cuda.synchronize()
+        start = (c.lengths.clone(), c.kp.clone(), c.vp.clone())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            outs = steps(c)
+        graphs.append((g, c, start, outs))
+    for _ in range(5):
+        for g, c, start, outs in graphs:
+            for x, y in zip((c.lengths, c.kp, c.vp), start):
+                x.copy_(y)
+        torch.cuda.synchronize()
+        for s, (g, c, start, outs) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for a, b, d in zip(want[i], other[i], graphs[i][3]):
+                assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+                assert torch.equal(a[0], d[0]) and torch.equal(a[1], d[1])
+    c = finals[0]
+    assert c.lengths.tolist() == [106, 903, 6, 37]
+    check_append(c, inv)
+    c.q = paged.append(c.q, c.k, c.v, *c.args(), inv, counts=c.counts)
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+def test_python_refusals(cuda_lib, dev):
+    from skinny_mlx_b200 import paged
+
+    c = Case(dev, [5, 9], T=2, Hq=4, Hkv=2)
+    ok = dict(q=c.q, k_pages=c.kp, v_pages=c.vp, block_table=c.table, lengths=c.lengths)
+    paged.attention(**ok)
+    i64 = c.lengths.long()
+    for bad in (dict(q=c.q.float()), dict(q=c.q[0]), dict(q=c.q[:1]), dict(q=c.q[..., :64]), dict(q=c.q[:, :, :3]), dict(q=c.q.cpu()),
+                dict(k_pages=c.kp.half()), dict(k_pages=c.kp[:, :1]), dict(k_pages=c.kp.transpose(1, 2)), dict(v_pages=c.vp.to(F8)),
+                dict(k_pages=c.kp.cpu(), v_pages=c.vp.cpu()), dict(block_table=c.table.long()), dict(block_table=c.table[:1]),
+                dict(block_table=c.table[:, :0]), dict(lengths=i64), dict(lengths=c.lengths[:1]), dict(counts=i64),
+                dict(counts=c.lengths.cpu()), dict(window=0), dict(k_scale=torch.ones(2, device=dev)),
+                dict(k_pages=c.kp.to(F8), v_pages=c.vp.to(F8)), dict(q=c.q.repeat(1, 9, 1, 1))):
+        with pytest.raises(ValueError):
+            paged.attention(**{**ok, **bad})
+    ok = dict(q=c.q, k=c.k, v=c.v, k_pages=c.kp, v_pages=c.vp, block_table=c.table, lengths=c.lengths, inv_freq=inv_freq(dev, 32))
+    paged.append(**ok)
+    for bad in (dict(k=c.k[:, :, :1]), dict(v=c.v[:, :1]), dict(k=c.k.float()), dict(inv_freq=inv_freq(dev, 20)),
+                dict(inv_freq=inv_freq(dev, 256)), dict(inv_freq=inv_freq(dev, 32).double()), dict(inv_freq=inv_freq("cpu", 32))):
+        with pytest.raises(ValueError):
+            paged.append(**{**ok, **bad})
+    # an empty batch and a step of no tokens are calls that do nothing
+    assert paged.attention(**{**dict(q=c.q[:, :0], k_pages=c.kp, v_pages=c.vp, block_table=c.table, lengths=c.lengths)}).shape == (2, 0, 4, 128)
+    z = dict(block_table=c.table[:0], lengths=c.lengths[:0], k_pages=c.kp, v_pages=c.vp)
+    assert paged.attention(q=c.q[:0], **z).shape == (0, 2, 4, 128)
+    assert paged.append(c.q[:0], c.k[:0], c.v[:0], **z).shape == (0, 2, 4, 128)
+    assert paged.device_errors(dev) == 0
