@@ -79,7 +79,7 @@ def test_append_entry_refuses(kw, status):
 
 @pytest.mark.parametrize("kw,status", COMMON + [
     (dict(q=None), -1), (dict(out=None), -1), (dict(window=-1), -1), (dict(T=0), -3), (dict(T=17), -3), (dict(Hq=3), -2),
-    (dict(Hq=0), -2), (dict(out=F + 8), -4), (dict(lse=F + 2), -4), (dict(ws=None), -5), (dict(wsn=0), -5), (dict(ws=F + 4), -5)])
+    (dict(Hq=0), -2), (dict(n=1 << 30), -2), (dict(vps=1 << 40), -2), (dict(out=F + 8), -4), (dict(lse=F + 2), -4), (dict(ws=None), -5), (dict(wsn=0), -5), (dict(ws=F + 4), -5)])
 def test_attention_entry_refuses(kw, status):
     assert _attn_status(**kw) == status
 
