@@ -661,8 +661,8 @@ int skinny_paged_attn(const void* q, const long long* q_strides, const void* k_p
   if (!out || window < 0) return SKINNY_ERR_INVALID_ARG;
   if (T < 1 || T > skinny::kPagedMaxTokens) return SKINNY_ERR_TOKENS;
   if (Hq < 1 || Hq % Hkv || static_cast<long long>(B) * T * Hq > INT32_MAX) return SKINNY_ERR_SHAPE;
-  // the kernel counts the pools' rows of D elements in 32 bits
-  if (n_pages > 0 && std::max(k_page_stride, v_page_stride) / D > (0xFFFFFFFFll - 1) / n_pages) return SKINNY_ERR_SHAPE;
+  // the copies' coordinate, a pool's row of D elements, is an int32
+  if (n_pages > 0 && std::max(k_page_stride, v_page_stride) / D > INT32_MAX / n_pages) return SKINNY_ERR_SHAPE;
   if (!aligned16(out) || !aligned4(lse)) return SKINNY_ERR_ALIGNMENT;
   st = paged_seqs(prm.seq, table, table_stride, width, n_pages, page, lengths, counts, B, T);
   if (st != SKINNY_OK) return st;

@@ -7,30 +7,35 @@
 //
 // One pass over the cache with a running maximum and sum, split over the cache's length and joined
 // (online softmax).  Bound by the bytes of the keys and values: each is read once from memory, by
-// one warp, straight into the registers that feed the matrix instructions.  Three choices make
-// that possible without shared memory or barriers in the loop:
+// the warp that multiplies it:
 //
 // * The keys are the 16-row operand and the query rows (t, head in the group; at most 8 NB of them)
 //   the 8-column operand: S^T[key][row] = K q^T, then O^T[dim][row] += V^T P^T.  A decode step has
 //   few rows, so 8-column tiles waste the least of the matrix unit, and O needs D / 16 * 4 registers
 //   per 8 rows.
-// * A dot product does not care in which order its dims come, so a thread's 16 consecutive bytes
-//   of a key row serve as its operand pieces of two (e4m3: four) consecutive 16-dim steps, and the
-//   query's fragments are loaded in the same order.  Likewise the 8 (16) consecutive dims a thread
-//   reads of a value row are its rows of 4 (8) output tiles; pairs of keys are interleaved with
-//   byte permutes.  Every load is 16 bytes and whole 32-byte sectors are used.
+// * Keys and values come by TMA, in boxes of up to 16 consecutive positions of a page (the largest
+//   power of two that divides the page size, so any page size works) x 128 bytes, swizzled, which
+//   makes the fragment loads below conflict-free.  The copy engine takes some 12 clocks per request
+//   whatever its size: one request per 256-byte row held the kernel at 5.9 TB/s, per 128-byte row at
+//   3.1.  A warp copies its own blocks and waits for them alone (one mbarrier per stage of keys and of
+//   values): the loop has no CTA barrier.  Ordinary asynchronous copies (16 bytes per lane) stood in
+//   the way of the shared-memory reads behind them in the same pipe: 4.3 TB/s.
+// * K fragments are ldmatrix rows.  e4m3 rows are read as pairs: a lane then holds 4 consecutive dims,
+//   two operand pieces of a 16-dim step in an order the query rows are stored in too (a dot product
+//   does not care).  V fragments: the 8 (16) consecutive dims a lane reads of a value row are its rows
+//   of 4 (8) output tiles; pairs of keys are interleaved with byte permutes.
 // * P^T as an operand is the transpose of the S^T accumulators, one movmatrix per 8 x 8 block.
 //
 // The maximum a row's exponentials refer to is renewed only when a score exceeds it by more than
 // 8 (in powers of two): p stays below 256, which bf16 and f16 hold at the same relative precision,
 // and the usual block needs one warp vote instead of shuffles and a rescaling of O.
-// Roundings: scores, maxima, sums and O are f32; p is rounded to bf16 (bf16 pages, 2^-9 of p on
-// average below the output's own rounding) or f16 (e4m3 pages: keys and values are exact in f16,
-// and q is scaled per row by a power of two so that it is exact too).  The sum adds the p before
-// that rounding, so the lse does not see it.
+// Roundings: scores, maxima, sums and O are f32; p is rounded to bf16 (bf16 pages: half a step, as
+// the output's own rounding) or f16 (e4m3 pages: keys and values are exact in f16, and q is scaled
+// per row by a power of two so that it is exact too).  The sum adds the p before that rounding, so
+// the lse does not see it.
 //
-// Work split: the tiles of 64 keys of all (sequence, kv head, row group) items form one line that
-// is cut into equal pieces, one per CTA (`kCtas` CTAs per SM), so that ragged lengths balance; the
+// Work split: the key tiles of all (sequence, kv head, row group) items form one line that is cut
+// into equal pieces, one per CTA (`kCtas` CTAs per SM), so that ragged lengths balance; the
 // lengths are read on the device and the launch does not depend on them (a captured graph serves
 // any).  A CTA whose piece covers an item writes its output; the others write (max, sum, O) to the
 // workspace and the join launch adds them in order, so results do not depend on timing.
@@ -40,8 +45,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "mma_bf16.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
 
@@ -49,11 +56,13 @@ namespace skinny {
 
 constexpr int kPtThreads = 128;
 constexpr int kPtWarps = kPtThreads / 32;
-constexpr int kPtTile = 64;               // keys of one unit of work: 16 per warp
 constexpr uint32_t kPtNone = 0xFFFFFFFFu;  // no such key (past the end, or a page outside the pool)
 constexpr float kPtSlack = 8.f;           // how far p may exceed 1, in powers of two
 
 struct PagedAttnPlan {
+  int tile;        // keys of one unit of work: one block per warp
+  int shift;       // log2 of the page size, or -1
+  int box;         // positions of one copy: the largest power of two up to 16 that divides the page size
   int nchunk;      // row chunks of 8 NB rows, one per warp (1, 2 or 4); the other warps split keys
   int groups;      // row groups of nchunk chunks per kv head
   int rows;        // rows of one group: 8 NB nchunk
@@ -65,16 +74,18 @@ struct PagedAttnPlan {
 
 // The positions some token of the sequence sees, and the tiles they make.
 struct PagedSpan {
-  int len, cnt, beg, end, tiles;
+  int len, cnt, beg, end;
+  int first, tiles;  // the tiles start at a multiple of 32: no box straddles two blocks
 };
 
-__device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, int b, bool* ok = nullptr) {
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, int b, int tile, bool* ok = nullptr) {
   PagedSpan s;
   const bool good = p.seq.get(b, s.len, s.cnt);
   if (ok) *ok = good;
   s.end = s.len + s.cnt;
   s.beg = p.window > 0 && s.len >= p.window ? s.len - p.window + 1 : 0;
-  s.tiles = s.cnt > 0 ? (s.end - s.beg + kPtTile - 1) / kPtTile : 0;
+  s.first = s.beg & ~31;
+  s.tiles = s.cnt > 0 ? (s.end - s.first + tile - 1) / tile : 0;
   return s;
 }
 
@@ -107,30 +118,42 @@ __device__ __forceinline__ void pt_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// WORDS 32-bit words at p, or zeros.  Volatile: the loads are issued where they stand.  (The pages
-// are not written while the kernel runs: non-coherent loads.)
-template <int WORDS>
-__device__ __forceinline__ void pt_load(uint32_t* r, const uint8_t* p, bool pred) {
-  if (WORDS == 4)
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
-        "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-        "@q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-        : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3])
-        : "l"(p), "r"(static_cast<uint32_t>(pred)));
-  else
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %3, 0;\n\t"
-        "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\t"
-        "@q ld.global.nc.v2.u32 {%0, %1}, [%2];\n\t}"
-        : "=&r"(r[0]), "=&r"(r[1])
-        : "l"(p), "r"(static_cast<uint32_t>(pred)));
+__device__ __forceinline__ void pt_lds4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void pt_lds2(uint32_t& x, uint32_t& y, uint32_t a) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(a) : "memory");
 }
 
-__device__ __forceinline__ uint32_t pt_cvt_e4m3x2(uint32_t pair) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair & 0xFFFFu), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+// Two pairs of e4m3 to two pairs of f16 (exact; NaN stays NaN).
+__device__ __forceinline__ void pt_cvt_e4m3(uint32_t& lo, uint32_t& hi, uint32_t x) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(x));
 }
+
+// a / b of non-negative numbers, in 32 bits where they fit.
+__device__ __forceinline__ long long pt_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The line's pieces: `total` tiles over `parts` CTAs, the first `rest` of them one tile longer.
+struct PtLine {
+  long long total, each, rest;
+  __device__ __forceinline__ PtLine(long long n, int ctas) : total(n), each(0), rest(0) {
+    const long long parts = min(n, static_cast<long long>(ctas));
+    if (parts > 0) {
+      each = pt_div(n, parts);
+      rest = n - each * parts;
+    }
+  }
+  __device__ __forceinline__ long long start(int i) const { return i * each + min(static_cast<long long>(i), rest); }
+  __device__ __forceinline__ int owner(long long u) const {
+    const long long longer = rest * (each + 1);
+    return static_cast<int>(u < longer ? pt_div(u, each + 1) : rest + pt_div(u - longer, each));
+  }
+};
 
 template <bool F16>
 __device__ __forceinline__ uint32_t pt_pack(float lo, float hi) {
@@ -142,42 +165,57 @@ __device__ __forceinline__ uint32_t pt_pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Sizes of one instance.  kCtas: CTAs per SM that the registers allow.
+// Sizes of one instance.
 template <int D, int NB, bool F8>
 struct PtShape {
-  static constexpr int kQWords = D / 8;                   // query fragment words per thread and 8 rows
-  static constexpr int kKWords = F8 ? D / 16 : D / 8;     // key words per thread and key (2 keys)
-  static constexpr int kPiece = F8 && D == 64 ? 2 : 4;    // words of one value load
-  static constexpr int kPieces = F8 ? (D + 127) / 128 : D / 64;  // value loads per thread and key (4 keys)
-  static constexpr int kElems = F8 ? 4 * kPiece : 8;      // consecutive dims of one value load
-  static constexpr int kTiles = D / 16;                   // output tiles of 16 dims
-  static constexpr bool kQRegs = NB * D <= (F8 || D < 256 ? 256 : 0);  // query fragments stay in registers
-  static constexpr int kCtas = NB * D <= 128 ? 3 : 2;
+  static constexpr int kEs = F8 ? 1 : 2;
+  // Keys of one block: 16, or 32 where a block of 16 would be less than 8 KB (the block's fixed
+  // instructions count for more then).
+  static constexpr int kSub = 16 * 2 * D * kEs < 8192 ? 2 : 1;
+  static constexpr int kKeys = 16 * kSub;
+  static constexpr int kRow = D * kEs;                           // bytes of a key or value row
+  static constexpr int kLine = kRow < 128 ? kRow : 128;          // bytes of it that one copy takes
+  static constexpr int kLines = kRow / kLine;
+  static constexpr int kQPad = 2 * D + 16;                       // bytes of a query row in shared memory (16-bit)
+  static constexpr int kQLoads = D / 32;                         // query fragment loads (4 words) per lane and 8 rows
+  static constexpr int kVBytes = F8 && D == 64 ? 8 : 16;         // bytes of one value fragment load
+  static constexpr int kVLoads = kRow / (8 * kVBytes);           // value fragment loads per lane and key (4 keys per 16)
+  static constexpr int kElems = kVBytes / kEs;                   // consecutive dims of one value load
+  static constexpr int kTiles = D / 16;                          // output tiles of 16 dims
+  static constexpr bool kQRegs = NB * D <= 256 && (F8 || D < 256);  // query fragments stay in registers
+  static constexpr int kCtas = NB * D <= 128 ? 3 : 2;            // CTAs per SM
+  static constexpr int kKBytes = kKeys * kRow;                   // keys (or values) of one block
+  static constexpr int kStages = 16384 / (2 * kKBytes);
+  static constexpr int kMaxNB = D <= 128 ? 4 : F8 ? 2 : 1;
+  static constexpr int kChunks = NB == kMaxNB ? kPtWarps : 1;    // row chunks a CTA may hold
+  static constexpr int kORow = D + 4;                            // floats of one row of O in shared memory
+  // a warp's region: its ring, later its O
+  static constexpr int kRing = kStages * 2 * kKBytes, kOBytes = 8 * NB * kORow * 4;
+  static constexpr int kWarpBytes = ((kRing > kOBytes ? kRing : kOBytes) + 1023) / 1024 * 1024;
+  static constexpr int kSmem = 1024 + kPtWarps * kWarpBytes + kChunks * 8 * NB * kQPad;
+  static_assert(kStages >= 1 && kKBytes % 1024 == 0, "a block starts on a swizzle period");
 };
 
 template <int D, int NB, bool F8>
-__host__ __device__ constexpr int pt_o_floats() { return kPtWarps * 8 * NB * (D + 4); }
-
-template <int D, int NB, bool F8>
-__host__ __device__ constexpr int pt_smem_bytes() {
-  using S = PtShape<D, NB, F8>;
-  return pt_o_floats<D, NB, F8>() * 4 + (S::kQRegs ? 0 : kPtWarps * NB * S::kQWords * 32 * 4);
-}
-
-template <int D, int NB, bool F8>
 __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
-    paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ PagedAttnPlan plan) {
+    paged_attn_split_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ PagedAttnPlan plan,
+                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using S = PtShape<D, NB, F8>;
-  constexpr int kEs = F8 ? 1 : 2;
-  extern __shared__ __align__(16) uint8_t pt_smem[];
-  float* const so = reinterpret_cast<float*>(pt_smem);                      // [warp][8 NB][D + 4]
-  uint32_t* const sq = reinterpret_cast<uint32_t*>(so + pt_o_floats<D, NB, F8>());  // [warp][NB][kQWords / 4][lane][4]
+  constexpr int kSub = S::kSub, kStages = S::kStages;
+  extern __shared__ __align__(1024) uint8_t pt_raw[];
+  uint8_t* const pt_smem = pt_raw + ((1024 - (smem_u32(pt_raw) & 1023)) & 1023);  // swizzle periods are 1 KB
+  __shared__ uint64_t bars[kPtWarps][kStages][2];  // per warp and stage: the keys are there, the values are there
+  __shared__ int gave_up;                          // a wait ran out
   __shared__ float sml[kPtWarps][8 * NB][2];
+  __shared__ float sdown[S::kChunks * 8 * NB];  // e4m3: the power of two each row's q was divided by
   __shared__ long long scan[kPtWarps];
   __shared__ long long found[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cq = lane & 3;
   const int rep = p.Hq / p.Hkv, items = p.Hkv * plan.groups, B = p.seq.B;
   pdl_launch_dependents();
+  if (tid < kPtWarps * kStages * 2) mbar_init(smem_u32(&bars[0][0][0]) + 8 * tid, 1);
+  if (tid == 0) gave_up = 0;
+  fence_mbar_init();
   pdl_wait_prior_grid();
 
   // ---- this CTA's piece of the line: thread i sums the tiles of its run of sequences
@@ -186,7 +224,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   bool all_ok = true;
   for (int b = b_lo; b < b_hi; ++b) {
     bool ok;
-    mine += static_cast<long long>(paged_span(p, b, &ok).tiles) * items;
+    mine += static_cast<long long>(paged_span(p, b, plan.tile, &ok).tiles) * items;
     all_ok &= ok;
   }
   long long incl = mine;
@@ -203,23 +241,23 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     if (w < warp) excl += scan[w];
     total += scan[w];
   }
-  const long long parts = min(static_cast<long long>(plan.ctas), total);
   if (blockIdx.x == 0) {  // the join's copy of the line
     long long at = excl;
     for (int b = b_lo; b < b_hi; ++b) {
       plan.pre[b] = at;
-      at += static_cast<long long>(paged_span(p, b).tiles) * items;
+      at += static_cast<long long>(paged_span(p, b, plan.tile).tiles) * items;
     }
     if (tid == 0) plan.pre[B] = total;
     if (!all_ok) atomicOr(p.seq.err, kErrBitBadInput);
   }
-  if (blockIdx.x >= parts) return;
-  long long u = blockIdx.x * total / parts;
-  const long long u_end = (blockIdx.x + 1ll) * total / parts;
+  if (blockIdx.x >= total) return;
+  const PtLine line(total, plan.ctas);
+  long long u = line.start(blockIdx.x);
+  const long long u_end = line.start(blockIdx.x + 1);
   if (excl <= u && u < excl + mine) {
     long long at = excl;
     for (int b = b_lo; b < b_hi; ++b) {
-      const long long n = static_cast<long long>(paged_span(p, b).tiles) * items;
+      const long long n = static_cast<long long>(paged_span(p, b, plan.tile).tiles) * items;
       if (u < at + n) {
         found[0] = b;
         found[1] = u - at;
@@ -233,61 +271,166 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   long long off = found[1];
   const int chunk = warp % plan.nchunk, slot = warp / plan.nchunk, slots = kPtWarps / plan.nchunk;
   const uint32_t kpr = static_cast<uint32_t>(p.kps / D), vpr = static_cast<uint32_t>(p.vps / D);
-  uint32_t* const myq = sq + static_cast<size_t>(warp) * NB * S::kQWords * 32 + lane * 4;
+  uint8_t* const region = pt_smem + warp * S::kWarpBytes;
+  float* const so = reinterpret_cast<float*>(region);                  // [8 NB][kORow], after the loop
+  const uint32_t ring = smem_u32(region);                               // [stage][keys | values][line][key][kLine], swizzled
+  const uint32_t bar0 = smem_u32(&bars[warp][0][0]);
+  // Fragment addresses inside a block.  Swizzle: 16-byte piece c of a 128-byte line of key k lies at
+  // c ^ (k & 7), of a 64-byte line at c ^ (k / 2 & 3).  K by ldmatrix: lanes 0-15 keys 0-15 at piece 2 i,
+  // lanes 16-31 at 2 i + 1 (the piece's step is an xor).  V: keys 2 cq + (e & 1) + 8 (e >> 1), dims from 8 g
+  // (16 g).
+  const uint32_t kkey = lane & 15, kswz = S::kLine == 128 ? kkey & 7 : kkey >> 1 & 3;
+  const uint32_t klane = kkey * S::kLine + ((static_cast<uint32_t>(lane >> 4) ^ kswz) << 4);
+  const uint32_t vlane0 = S::kLine == 128 ? 2 * cq * 128 + ((g ^ (2 * cq)) << 4)
+                                          : 2 * cq * 64 + (((g >> 1) ^ cq) << 4) + (g & 1) * 8;
+  const uint32_t vlane1 = S::kLine == 128 ? (vlane0 ^ 16) + 128 : vlane0 + 64;  // the odd keys
+  uint8_t* const sq = pt_smem + kPtWarps * S::kWarpBytes;               // [chunk][8 NB][kQPad]
+  int stage = 0;                       // of the next block to multiply
+  uint32_t pending = 0, parity = 0;    // per barrier (bit 2 stage + what): copies in flight, the phase they complete
   bool bad = false;
 
   for (int seg = 0; u < u_end; ++seg) {
-    const PagedSpan sp = paged_span(p, b);
+    const PagedSpan sp = paged_span(p, b, plan.tile);
     if (sp.tiles == 0) {
       ++b;
       --seg;
       continue;
     }
-    const int item = static_cast<int>(off / sp.tiles), t0 = static_cast<int>(off - static_cast<long long>(item) * sp.tiles);
+    const int item = static_cast<int>(pt_div(off, sp.tiles)), t0 = static_cast<int>(off - static_cast<long long>(item) * sp.tiles);
     const int t1 = static_cast<int>(min(static_cast<long long>(sp.tiles), t0 + (u_end - u)));
     const int kvh = item / plan.groups, rbase = (item % plan.groups) * plan.rows;
-    const int k0 = sp.beg + t0 * kPtTile, k1 = min(sp.end, sp.beg + t1 * kPtTile);
+    const int k0 = sp.first + t0 * plan.tile, k1 = min(sp.end, sp.first + t1 * plan.tile);
     const int r0 = rbase + chunk * 8 * NB;  // this warp's first row
     const int32_t* const table = p.seq.table + b * p.seq.table_stride;
 
-    // ---- query fragments; sc: the factor that takes a score to powers of two
-    uint32_t qr[S::kQRegs ? NB : 1][S::kQRegs ? S::kQWords : 1];
-    float sc[F8 ? NB : 1][2];
-    const float sc0 = p.scale * 1.4426950408889634f * (F8 ? p.k_scale[kvh] : 1.f);
-    if (!F8) sc[0][0] = sc0;
+    // ---- this warp's blocks of keys: block n holds the keys from k0 + kKeys (n slots + slot)
+    const int nblk_all = (k1 - k0 + S::kKeys - 1) / S::kKeys;
+    const int nblk = nblk_all > slot ? (nblk_all - slot + slots - 1) / slots : 0;
+    const auto first_key = [&](int n) { return k0 + S::kKeys * (n * slots + slot); };
+    // a block's pages, one key per lane (16 keys: lanes 16..31 repeat), and from them its rows
+    const auto page_of = [&](int n, int& in_page) {
+      const int j = first_key(n) + (lane & (S::kKeys - 1));
+      if (n >= nblk || j < sp.beg || j >= k1) return -2;
+      const int q = plan.shift >= 0 ? j >> plan.shift : j / p.seq.page;
+      in_page = j - q * p.seq.page;
+      return __ldg(table + q);
+    };
+    uint32_t rk, rv;
+    const auto rows_of = [&](int pid, int in_page) {  // -> the keys that exist, one bit each
+      const bool ok = pid >= 0 && pid < p.seq.n_pages;
+      bad |= !ok && pid != -2;
+      const uint32_t at = static_cast<uint32_t>(kvh) * p.seq.page + static_cast<uint32_t>(in_page);
+      rk = ok ? static_cast<uint32_t>(pid) * kpr + at : kPtNone;
+      rv = ok ? static_cast<uint32_t>(pid) * vpr + at : kPtNone;
+      return __ballot_sync(0xFFFFFFFFu, ok);
+    };
+    // The block whose pages were looked up last (one key per lane) into stage st, one box per lane; its
+    // slots have been read by all lanes.  A box without a key that exists is left out.
+    const auto copy = [&](int st, int what, uint32_t r, uint32_t exist) {
+      const uint32_t bar = bar0 + (st * 2 + what) * 8;
+      const int first = lane * plan.box;
+      const uint32_t here = first < S::kKeys ? exist & ((1u << plan.box) - 1u) << first : 0u;
+      const int src = here ? __ffs(here) - 1 : 0;
+      const uint32_t row = __shfl_sync(0xFFFFFFFFu, r, src) - static_cast<uint32_t>(src - first);
+      const int boxes = __popc(__ballot_sync(0xFFFFFFFFu, here != 0));
+      if (lane == 0) mbar_arrive_expect_tx(bar, boxes * plan.box * S::kRow);
+      __syncwarp();
+      if (here) {
+        const uint32_t dst = ring + (st * 2 + what) * S::kKBytes + first * S::kLine;
+        if (S::kLine == 64 && plan.box == 1) {  // 64 bytes: less than a tiled copy's alignment
+          const uint8_t* const from = static_cast<const uint8_t*>(what ? p.vp : p.kp) + static_cast<size_t>(row) * S::kRow;
+          for (int c = 0; c < 4; ++c) bulk_g2s(dst + ((c ^ (first >> 1 & 3)) << 4), from + 16 * c, 16, bar);
+        } else {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int r = r0 + 8 * nb + g, t = r / rep, h = kvh * rep + r % rep;
-      const bool live = t < sp.cnt;
-      const uint8_t* const src =
-          reinterpret_cast<const uint8_t*>(p.q + b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) + cq * (F8 ? 32 : 16);
-      uint32_t w[S::kQWords];
-#pragma unroll
-      for (int i = 0; i < S::kQWords / 4; ++i)
-        pt_load<4>(w + 4 * i, src + (F8 ? (i >> 1) * 128 + (i & 1) * 16 : i * 64), live);
-      if (F8) {  // to f16, the row's largest |q| to [1, 2)
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < S::kQWords; ++i) top = max(top, max(w[i] & 0x7FFFu, (w[i] >> 16) & 0x7FFFu));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        const uint32_t ex = min(max(top >> 7, 1u), 253u);
-        const float up = top >= 0x7F80u ? 1.f : __uint_as_float((254u - ex) << 23);
-        const float down = top >= 0x7F80u ? 1.f : __uint_as_float(ex << 23);
-#pragma unroll
-        for (int i = 0; i < S::kQWords; ++i)
-          w[i] = pt_pack<true>(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xFFFF0000u) * up);
-        sc[nb][0] = sc0 * __shfl_sync(0xFFFFFFFFu, down, 8 * cq);  // rows 2 cq and 2 cq + 1: lanes g = row
-        sc[nb][1] = sc0 * __shfl_sync(0xFFFFFFFFu, down, 8 * cq + 4);
+          for (int c = 0; c < S::kLines; ++c)
+            tma_load_2d(dst + c * (S::kKeys * S::kLine), what ? &vmap : &kmap, c * (S::kLine / S::kEs), static_cast<int>(row), bar);
+        }
       }
+      pending |= 1u << (st * 2 + what);
+    };
+    const auto arrived = [&](int st, int what) {  // bounded; the same answer in every lane
+      const int bit = st * 2 + what;
+      const bool ok = mbar_wait(bar0 + bit * 8, parity >> bit & 1u, p.seq.err, kErrBitWaitFull, &gave_up);
+      if (!__all_sync(0xFFFFFFFFu, ok)) return false;
+      pending &= ~(1u << bit);
+      parity ^= 1u << bit;
+      return true;
+    };
+    uint32_t have[kStages];  // the keys that exist of the blocks in flight
+    int pid_next, in_next = 0;
+    {
+      int pid[kStages], in[kStages];
 #pragma unroll
-      for (int i = 0; i < S::kQWords; ++i) {
-        if (S::kQRegs) qr[nb][i] = w[i];
-        else myq[(nb * S::kQWords / 4 + i / 4) * 128 + i % 4] = w[i];
+      for (int st = 0; st < kStages; ++st) {
+        in[st] = 0;
+        pid[st] = page_of(st, in[st]);
+      }
+      pid_next = page_of(kStages, in_next);
+      fence_proxy_async_smem();  // the previous segment's O was written here by ordinary stores
+      __syncthreads();           // and has been read
+#pragma unroll
+      for (int st = 0; st < kStages; ++st) {
+        have[st] = rows_of(pid[st], in[st]);
+        if (st < nblk) {
+          const int at = stage + st < kStages ? stage + st : stage + st - kStages;
+          copy(at, 0, rk, have[st]);
+          copy(at, 1, rv, have[st]);
+        }
       }
     }
 
-    // ---- one pass over the keys of the segment: 16-key blocks slot, slot + slots, ...
+    // ---- the query rows to shared memory, 8 dims per thread at a time
+    const float sc0 = p.scale * 1.4426950408889634f * (F8 ? p.k_scale[kvh] : 1.f);
+    for (int e = tid; e < plan.rows * (D / 8); e += kPtThreads) {
+      const int row = e / (D / 8), u8 = e % (D / 8);
+      const int r = rbase + row, t = r / rep, h = kvh * rep + r % rep;
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (t < sp.cnt) w = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) + u8);
+      uint8_t* const dst = sq + row * S::kQPad;
+      if (F8) {  // to f16, the row's largest |q| to [1, 2); pairs 0, 2, .. of 16 dims before pairs 1, 3, ..
+        uint32_t x[4] = {w.x, w.y, w.z, w.w}, top = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top = max(top, max(x[c] & 0x7FFFu, (x[c] >> 16) & 0x7FFFu));
+#pragma unroll
+        for (int o = 1; o < D / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const uint32_t ex = min(max(top >> 7, 1u), 253u);
+        const float up = top >= 0x7F80u ? 1.f : __uint_as_float((254u - ex) << 23);
+        if (u8 == 0) sdown[row] = top >= 0x7F80u ? 1.f : __uint_as_float(ex << 23);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<uint32_t*>(dst + (u8 >> 1) * 32 + (c & 1) * 16 + (u8 & 1) * 8 + (c >> 1) * 4) =
+              pt_pack<true>(__uint_as_float(x[c] << 16) * up, __uint_as_float(x[c] & 0xFFFF0000u) * up);
+      } else {
+        reinterpret_cast<uint4*>(dst)[u8] = w;
+      }
+    }
+    __syncthreads();
+    // fragments by ldmatrix: rows 0-7 of a block at 16-byte pieces 4 i .. 4 i + 3
+    const uint32_t qaddr = smem_u32(sq) + (chunk * 8 * NB + (lane & 7)) * S::kQPad + (lane >> 3) * 16;
+    // and where they do not stay in registers, one 16-dim step of two blocks (of one block)
+    const uint32_t qaddr_2 = smem_u32(sq) + (chunk * 8 * NB + (lane & 7) + 8 * (lane >> 4)) * S::kQPad + ((lane >> 3) & 1) * 16;
+    const uint32_t qaddr_x2 = smem_u32(sq) + (chunk * 8 * NB + (lane & 7)) * S::kQPad + ((lane >> 3) & 1) * 16;
+    uint32_t qr[S::kQRegs ? NB : 1][S::kQRegs ? S::kQLoads : 1][4];
+    if (S::kQRegs) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < S::kQLoads; ++i) {
+          uint32_t(&x)[4] = qr[S::kQRegs ? nb : 0][S::kQRegs ? i : 0];
+          ldsm_x4(qaddr + nb * 8 * S::kQPad + i * 64, x[0], x[1], x[2], x[3]);
+        }
+    }
+    float sc[F8 ? NB : 1][2];  // the factor that takes a score to powers of two
+    if (F8) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sc[F8 ? nb : 0][e] = sc0 * sdown[chunk * 8 * NB + 8 * nb + 2 * cq + e];
+    } else {
+      sc[0][0] = sc[0][1] = sc0;
+    }
+
+    // ---- one pass over the blocks
     float o[NB][S::kTiles][4], m[NB][2], l[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -298,115 +441,103 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nb][i][e] = 0.f;
     }
-    const int nblk = (k1 - k0 + 15) >> 4;
-    uint32_t kw[2][S::kKWords], vw[4][S::kPieces * S::kPiece];
-    // a block's page ids, one per lane (lanes 16..31 repeat), and from them its rows in the pools
-    const auto page_id = [&](int i) {
-      const int j = k0 + 16 * i + (lane & 15);
-      return i < nblk && j < k1 ? __ldg(table + j / p.seq.page) : -1;
+    const auto sees = [&](int row, int j) {  // does row r0 + row see position j
+      const int pos = sp.len + (r0 + row) / rep;
+      return j <= pos && (p.window <= 0 || j > pos - p.window);
     };
-    const auto row_of = [&](int i, int pid, uint32_t& rk, uint32_t& rv) {
-      const int j = k0 + 16 * i + (lane & 15);
-      const bool in = i < nblk && j < k1, ok = in && pid >= 0 && pid < p.seq.n_pages;
-      bad |= in && !ok;
-      const uint32_t in_page = static_cast<uint32_t>(kvh) * p.seq.page + static_cast<uint32_t>(j % p.seq.page);
-      rk = ok ? static_cast<uint32_t>(pid) * kpr + in_page : kPtNone;
-      rv = ok ? static_cast<uint32_t>(pid) * vpr + in_page : kPtNone;
+    const auto is_edge = [&](int j0) {  // a block that some row sees only part of
+      return j0 + S::kKeys - 1 > sp.len || (p.window > 0 && j0 <= sp.len + sp.cnt - 1 - p.window);
     };
-    const auto load_k = [&](uint32_t rk) {
+    bool poison = false;
+    for (int n = 0; n < nblk; ++n) {
+      const int j0 = first_key(n);
+      const uint32_t kaddr = ring + stage * (2 * S::kKBytes) + klane;
+      const uint32_t vblock = ring + stage * (2 * S::kKBytes) + S::kKBytes;
+      const uint32_t now = have[0];
+      const uint32_t have_next = rows_of(pid_next, in_next);
+      pid_next = page_of(n + kStages + 1, in_next);
+      // scores S^T = K q^T: s[nb][sub] = (key g: rows 2 cq, 2 cq + 1; key g + 8: the same rows)
+      float s[NB][kSub][4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t r = __shfl_sync(0xFFFFFFFFu, rk, g + 8 * e);
-        const uint8_t* const src = static_cast<const uint8_t*>(p.kp) + static_cast<size_t>(r) * (D * kEs) + cq * 16;
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int i = 0; i < S::kKWords / 4; ++i) pt_load<4>(kw[e] + 4 * i, src + i * 64, r != kPtNone);
-      }
-    };
-    const auto load_v = [&](uint32_t rv) {
+        for (int sub = 0; sub < kSub; ++sub) s[nb][sub][0] = s[nb][sub][1] = s[nb][sub][2] = s[nb][sub][3] = 0.f;
+      if (!arrived(stage, 0)) break;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t r = __shfl_sync(0xFFFFFFFFu, rv, 2 * cq + (e & 1) + 8 * (e >> 1));
-        const uint8_t* const src =
-            static_cast<const uint8_t*>(p.vp) + static_cast<size_t>(r) * (D * kEs) + g * (S::kElems * kEs);
+      for (int i = 0; i < S::kRow / 32; ++i) {  // 32 bytes of 16 (32) keys: one 16-dim step, or two of e4m3
+        uint32_t kw[kSub][4];
 #pragma unroll
-        for (int i = 0; i < S::kPieces; ++i)
-          pt_load<S::kPiece>(vw[e] + S::kPiece * i, src + i * (8 * S::kElems * kEs), r != kPtNone);
-      }
-    };
-    uint32_t rk, rv, rk_next = kPtNone, rv_next = kPtNone;
-    int pid = page_id(slot), pid_next = page_id(slot + slots);
-    row_of(slot, pid, rk, rv);
-    if (slot < nblk) {
-      load_k(rk);
-      load_v(rv);
-    }
-    for (int i = slot; i < nblk; i += slots) {
-      const int j0 = k0 + 16 * i;
-      row_of(i + slots, pid_next, rk_next, rv_next);
-      pid_next = page_id(i + 2 * slots);
-      // scores S^T = K q^T: s[nb] = (key g: rows 2 cq, 2 cq + 1; key g + 8: the same rows)
-      float s[NB][4];
+        for (int sub = 0; sub < kSub; ++sub)
+          ldsm_x4((kaddr ^ (i * 32 % S::kLine)) + i * 32 / S::kLine * (S::kKeys * S::kLine) + sub * 16 * S::kLine, kw[sub][0],
+                  kw[sub][1], kw[sub][2], kw[sub][3]);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+        for (int c = 0; c < (F8 ? 2 : 1); ++c) {
+          const int ks = F8 ? 2 * i + c : i;
+          uint32_t bq[NB][2];
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t a0, a1, a2, a3;
-        if (F8) {
-          a0 = pt_cvt_e4m3x2(kw[0][F8 ? ks : 0]);
-          a1 = pt_cvt_e4m3x2(kw[1][F8 ? ks : 0]);
-          a2 = pt_cvt_e4m3x2(kw[0][F8 ? ks : 0] >> 16);
-          a3 = pt_cvt_e4m3x2(kw[1][F8 ? ks : 0] >> 16);
-        } else {
-          a0 = kw[0][F8 ? 0 : 2 * ks];
-          a1 = kw[1][F8 ? 0 : 2 * ks];
-          a2 = kw[0][F8 ? 0 : 2 * ks + 1];
-          a3 = kw[1][F8 ? 0 : 2 * ks + 1];
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          uint32_t b0, b1;
-          if (S::kQRegs) {
-            b0 = qr[S::kQRegs ? nb : 0][S::kQRegs ? 2 * ks : 0];
-            b1 = qr[S::kQRegs ? nb : 0][S::kQRegs ? 2 * ks + 1 : 0];
-          } else {
-            const uint2 q2 =
-                *reinterpret_cast<const uint2*>(myq + (nb * S::kQWords / 4 + ks / 2) * 128 + (ks % 2) * 2);
-            b0 = q2.x;
-            b1 = q2.y;
+          for (int nb = 0; nb < NB; ++nb) {
+            if (S::kQRegs) {
+              bq[nb][0] = qr[S::kQRegs ? nb : 0][S::kQRegs ? ks / 2 : 0][(ks & 1) * 2];
+              bq[nb][1] = qr[S::kQRegs ? nb : 0][S::kQRegs ? ks / 2 : 0][(ks & 1) * 2 + 1];
+            }
           }
-          pt_mma<F8>(s[nb], a0, a1, a2, a3, b0, b1);
+          if (!S::kQRegs) {
+            if (NB == 1) {
+              ldsm_x2(qaddr_x2 + ks * 32, bq[0][0], bq[0][1]);
+            } else {
+#pragma unroll
+              for (int nb = 0; nb < NB; nb += 2)
+                ldsm_x4(qaddr_2 + nb * 8 * S::kQPad + ks * 32, bq[nb][0], bq[nb][1], bq[(nb + 1) % NB][0], bq[(nb + 1) % NB][1]);
+            }
+          }
+#pragma unroll
+          for (int sub = 0; sub < kSub; ++sub) {
+            uint32_t a0, a1, a2, a3;  // (keys 0-7, 8-15) x (first, second half of the step)
+            if (F8) {
+              pt_cvt_e4m3(a0, a2, kw[sub][2 * c]);
+              pt_cvt_e4m3(a1, a3, kw[sub][2 * c + 1]);
+            } else {
+              a0 = kw[sub][0];
+              a1 = kw[sub][1];
+              a2 = kw[sub][2];
+              a3 = kw[sub][3];
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) pt_mma<F8>(s[nb][sub], a0, a1, a2, a3, bq[nb][0], bq[nb][1]);
+          }
         }
       }
-      if (i + slots < nblk) load_k(rk_next);
-      // a block that not every row sees whole: past some row's position, before some row's window,
-      // or with keys that do not exist
-      const bool edge = j0 + 15 > sp.len || (p.window > 0 && j0 <= sp.len + sp.cnt - 1 - p.window) ||
-                        __any_sync(0xFFFFFFFFu, rk == kPtNone);
-      const auto sees = [&](int nb, int e, int key) {  // row 2 cq + e of block nb, key of this block
-        const int pos = sp.len + (r0 + 8 * nb + 2 * cq + e) / rep, j = j0 + key;
-        return j <= pos && (p.window <= 0 || j > pos - p.window);
-      };
+      if (n + kStages < nblk) copy(stage, 0, rk, have_next);
+      constexpr uint32_t kAll = 0xFFFFFFFFu;
+      const bool edge = is_edge(j0) || now != kAll;
       bool up = false;
-      uint32_t have = 0;
-      if (edge) have = __ballot_sync(0xFFFFFFFFu, rk != kPtNone);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[nb][e] *= F8 ? sc[F8 ? nb : 0][e & 1] : sc[0][0];
-          if (edge) {
-            const int key = g + 8 * (e >> 1);
-            if (!(have >> key & 1u) || !sees(nb, e & 1, key)) s[nb][e] = -INFINITY;
-          }
+        for (int e = 0; e < 2; ++e) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              float& x = s[nb][sub][2 * hf + e];
+              x *= sc[F8 ? nb : 0][e];
+              if (edge) {
+                const int key = 16 * sub + 8 * hf + g;
+                if (!(now >> key & 1u) || !sees(8 * nb + 2 * cq + e, j0 + key)) x = -INFINITY;
+              }
+              top = fmaxf(top, x);
+            }
+          up |= top > m[nb][e] + kPtSlack;
         }
-        up |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kPtSlack || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kPtSlack;
-      }
       if (__any_sync(0xFFFFFFFFu, up)) {  // renew the maxima, rescale the sums
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(m[nb][e], fmaxf(s[nb][e], s[nb][2 + e]));
+            float x = m[nb][e];
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub) x = fmaxf(x, fmaxf(s[nb][sub][e], s[nb][sub][2 + e]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, w));
             const float f = m[nb][e] == x ? 1.f : pt_exp2(m[nb][e] - x);
@@ -419,105 +550,107 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
             }
           }
       }
-      uint32_t pb[NB][2];
+      uint32_t pb[NB][kSub][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
-        s[nb][0] = pt_exp2(s[nb][0] - m0);
-        s[nb][1] = pt_exp2(s[nb][1] - m1);
-        s[nb][2] = pt_exp2(s[nb][2] - m0);
-        s[nb][3] = pt_exp2(s[nb][3] - m1);
-        l[nb][0] += s[nb][0] + s[nb][2];
-        l[nb][1] += s[nb][1] + s[nb][3];
-        pb[nb][0] = pt_transpose(pt_pack<F8>(s[nb][0], s[nb][1]));
-        pb[nb][1] = pt_transpose(pt_pack<F8>(s[nb][2], s[nb][3]));
-      }
-      // An infinity or NaN among values that some row does not see would reach it as 0 * inf: such a
-      // block (only where tokens of one draft see different keys) is added key by key instead.
-      bool apart = false;
-      if (edge && p.seq.T > 1) {
-        bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int i2 = 0; i2 < S::kPieces * S::kPiece; ++i2) {
-            const uint32_t x = vw[e][i2];
-            if (F8) odd |= __vcmpeq4(x & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
-            else odd |= (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
-          }
-        apart = __any_sync(0xFFFFFFFFu, odd);
-      }
-      if (!apart) {  // O^T += V^T P^T
-#pragma unroll
-        for (int i2 = 0; i2 < S::kPieces * S::kPiece; ++i2) {
-          const uint32_t v0 = vw[0][i2], v1 = vw[1][i2], v2 = vw[2][i2], v3 = vw[3][i2];
-          if (F8) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const uint32_t x = __byte_perm(v0, v1, hf ? 0x7362 : 0x5140), y = __byte_perm(v2, v3, hf ? 0x7362 : 0x5140);
-              const uint32_t a0 = pt_cvt_e4m3x2(x), a1 = pt_cvt_e4m3x2(x >> 16), a2 = pt_cvt_e4m3x2(y),
-                             a3 = pt_cvt_e4m3x2(y >> 16);
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) pt_mma<true>(o[nb][F8 ? 2 * i2 + hf : 0], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
-            }
-          } else {
-            const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632),
-                           a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) pt_mma<false>(o[nb][F8 ? 0 : i2], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
-          }
+        for (int sub = 0; sub < kSub; ++sub) {
+          float(&x)[4] = s[nb][sub];
+          x[0] = pt_exp2(x[0] - m0);
+          x[1] = pt_exp2(x[1] - m1);
+          x[2] = pt_exp2(x[2] - m0);
+          x[3] = pt_exp2(x[3] - m1);
+          l[nb][0] += x[0] + x[2];
+          l[nb][1] += x[1] + x[3];
+          pb[nb][sub][0] = pt_transpose(pt_pack<F8>(x[0], x[1]));
+          pb[nb][sub][1] = pt_transpose(pt_pack<F8>(x[2], x[3]));
         }
-      } else {
+      }
+      if (!arrived(stage, 1)) break;
+      if (now != kAll) {  // keys that do not exist multiply zeros
+        if (lane < S::kKeys && !(now >> lane & 1u))
+#pragma unroll
+          for (int c = 0; c < S::kLines; ++c)
+#pragma unroll
+            for (int i = 0; i < S::kLine; i += 16)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vblock + (c * S::kKeys + lane) * S::kLine + i),
+                           "r"(0u)
+                           : "memory");
+        fence_proxy_async_smem();  // (the slot's next copy is ordered after these stores)
+        __syncwarp();
+      }
+      // An infinity or NaN among values that some row does not see would reach it as 0 * inf.  Such a
+      // block (only where tokens of one draft see different keys) multiplies zeros in their place;
+      // the rows that do see them get them after the loop.
+      if (p.seq.T > 1 && is_edge(j0)) {
+        bool odd = false;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c)  // keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9: held by the lanes (g, c)
+        for (int q = lane * 8; q < S::kKeys * S::kRow; q += 256) {
+          const uint32_t a = vblock + q;
+          uint32_t x[2];
+          pt_lds2(x[0], x[1], a);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t mask = F8 ? __vcmpeq4(x[c] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) : __vcmpeq2(x[c] & 0x7F807F80u, 0x7F807F80u);
+            odd |= mask != 0;
+            x[c] &= ~mask;
+          }
+          if (odd) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x[0]), "r"(x[1]) : "memory");
+        }
+        fence_proxy_async_smem();
+        poison |= __any_sync(0xFFFFFFFFu, odd);
+        __syncwarp();
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+        for (int i = 0; i < S::kVLoads; ++i) {
+          uint32_t v[4][4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int key = 2 * c + (e & 1) + 8 * (e >> 1);
-            float pk[NB][2];
+            const uint32_t a = vblock + (e & 1 ? vlane1 : vlane0) + ((e >> 1) * 8 + 16 * sub + i * S::kKeys) * S::kLine;
+            if (S::kVBytes == 16) pt_lds4(v[e], a);
+            else pt_lds2(v[e][0], v[e][1], a);
+          }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+          for (int c = 0; c < S::kVBytes / 4; ++c) {
+            if (F8) {
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                pk[nb][q] = __shfl_sync(0xFFFFFFFFu, s[nb][(e >> 1) * 2 + q], (2 * c + (e & 1)) * 4 + cq);
-                if (!(have >> key & 1u) || !sees(nb, q, key)) pk[nb][q] = -1.f;
+              for (int hf = 0; hf < 2; ++hf) {
+                uint32_t a0, a1, a2, a3;
+                pt_cvt_e4m3(a0, a1, __byte_perm(v[0][c], v[1][c], hf ? 0x7362 : 0x5140));
+                pt_cvt_e4m3(a2, a3, __byte_perm(v[2][c], v[3][c], hf ? 0x7362 : 0x5140));
+                const int q = F8 ? 2 * (i * (S::kVBytes / 4) + c) + hf : 0;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) pt_mma<true>(o[nb][q], a0, a1, a2, a3, pb[nb][sub][0], pb[nb][sub][1]);
               }
+            } else {
+              const uint32_t a0 = __byte_perm(v[0][c], v[1][c], 0x5410), a1 = __byte_perm(v[0][c], v[1][c], 0x7632),
+                             a2 = __byte_perm(v[2][c], v[3][c], 0x5410), a3 = __byte_perm(v[2][c], v[3][c], 0x7632);
+              const int q = F8 ? 0 : 4 * i + c;
 #pragma unroll
-            for (int i2 = 0; i2 < S::kPieces * S::kPiece; ++i2) {
-              const uint32_t x = __shfl_sync(0xFFFFFFFFu, vw[e][i2], g * 4 + c);
-              float v[F8 ? 4 : 2];
-              if (F8) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                  const uint32_t hh = pt_cvt_e4m3x2(x >> (16 * q));
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh));
-                  v[F8 ? 2 * q : 0] = f.x;
-                  v[F8 ? 2 * q + 1 : 1] = f.y;
-                }
-              } else {
-                v[0] = __uint_as_float(x << 16);
-                v[1] = __uint_as_float(x & 0xFFFF0000u);
-              }
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-                  if (pk[nb][q] >= 0.f || pk[nb][q] != pk[nb][q]) {
-#pragma unroll
-                    for (int d = 0; d < (F8 ? 4 : 2); ++d) {
-                      float& acc = o[nb][F8 ? 2 * i2 + (d >> 1) : i2][2 * (d & 1) + q];
-                      acc = fmaf(pk[nb][q], v[d], acc);
-                    }
-                  }
+              for (int nb = 0; nb < NB; ++nb) pt_mma<false>(o[nb][q], a0, a1, a2, a3, pb[nb][sub][0], pb[nb][sub][1]);
             }
           }
-      }
-      if (i + slots < nblk) load_v(rv_next);
-      rk = rk_next;
-      rv = rv_next;
+        }
+      if (n + kStages < nblk) copy(stage, 1, rv, have_next);
+#pragma unroll
+      for (int st = 0; st + 1 < kStages; ++st) have[st] = have[st + 1];
+      have[kStages - 1] = have_next;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    if (pending) {  // gave up: no copy may land after the CTA has left (bounded again)
+      const uint64_t t0 = globaltimer_ns();
+      for (int bit = 0; bit < 2 * kStages; ++bit)
+        while ((pending >> bit & 1u) && !mbar_try_wait(bar0 + bit * 8, parity >> bit & 1u) &&
+               globaltimer_ns() - t0 < SKINNY_WAIT_NS) {
+        }
     }
 
-    // ---- the warps' results: (maximum, sum) and O to shared memory, joined by all threads
-    __syncthreads();  // the previous segment's reads are done
+    // ---- the warps' results: (maximum, sum) and O to shared memory, joined row by row
+    __syncwarp();  // the ring's slots of all lanes are free
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -529,46 +662,87 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
           sml[warp][r][0] = m[nb][e];
           sml[warp][r][1] = l[nb][e];
         }
-        float* const dst = so + (warp * 8 * NB + r) * (D + 4);
+        float* const dst = so + r * S::kORow;
 #pragma unroll
         for (int q = 0; q < S::kTiles; q += 2) {  // two tiles: 4 consecutive dims
-          const int per = S::kElems / 2, piece = q / per, in = q % per;
-          *reinterpret_cast<float4*>(dst + piece * 8 * S::kElems + g * S::kElems + 2 * in) =
+          constexpr int per = S::kElems / 2;
+          *reinterpret_cast<float4*>(dst + (q / per) * 8 * S::kElems + g * S::kElems + 2 * (q % per)) =
               make_float4(o[nb][q][e], o[nb][q][2 + e], o[nb][q + 1][e], o[nb][q + 1][2 + e]);
         }
       }
+    if (poison) {  // the infinities and NaN that were left out, to the rows that see them
+      __syncwarp();
+#pragma unroll 1
+      for (int n = 0; n < nblk; ++n) {
+        const int j0 = first_key(n);
+#pragma unroll 1
+        for (int j = j0; is_edge(j0) && j < min(j0 + S::kKeys, k1); ++j) {
+          const int pid = table[j / p.seq.page];
+          if (pid < 0 || pid >= p.seq.n_pages) continue;
+          const size_t at = pid * static_cast<size_t>(p.vps) + (static_cast<size_t>(kvh) * p.seq.page + j % p.seq.page) * D;
+#pragma unroll 1
+          for (int d = lane; d < D; d += 32) {
+            float v;
+            if (F8) {
+              __nv_fp8_e4m3 x;
+              x.__x = static_cast<const uint8_t*>(p.vp)[at + d];
+              v = static_cast<float>(x);
+            } else {
+              v = __bfloat162float(static_cast<const __nv_bfloat16*>(p.vp)[at + d]);
+            }
+            if (!isfinite(v))
+#pragma unroll 1
+              for (int r = 0; r < 8 * NB; ++r)
+                if (sees(r, j)) so[r * S::kORow + d] += v;
+          }
+        }
+      }
+    }
     __syncthreads();
     const bool whole = t0 == 0 && t1 == sp.tiles;
     const size_t piece = 2 * static_cast<size_t>(blockIdx.x) + (seg > 0);
     const float vs = F8 ? p.v_scale[kvh] : 1.f;
     const int live = min(plan.rows, sp.cnt * rep - rbase);  // rows of the group that exist
-    for (int e = tid; e < live * (D / 4); e += kPtThreads) {
-      const int r = e / (D / 4), d = (e % (D / 4)) * 4, c = r / (8 * NB), rr = r % (8 * NB);
-      float mx = -INFINITY;
-      for (int w = c; w < kPtWarps; w += plan.nchunk) mx = fmaxf(mx, sml[w][rr][0]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-      for (int w = c; w < kPtWarps; w += plan.nchunk) {
-        const float f = sml[w][rr][0] == mx ? 1.f : pt_exp2(sml[w][rr][0] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 * NB + rr) * (D + 4) + d);
-        sum = fmaf(f, sml[w][rr][1], sum);
-        acc.x = fmaf(f, x.x, acc.x);
-        acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z);
-        acc.w = fmaf(f, x.w, acc.w);
+    for (int r = warp; r < live; r += kPtWarps) {
+      const int c = r / (8 * NB), rr = r % (8 * NB);
+      float ml[kPtWarps][2], mx = -INFINITY, sum = 0.f;  // over the warps of the row's chunk
+#pragma unroll
+      for (int w = 0; w < kPtWarps; ++w) {
+        const bool on = w < slots;
+        ml[w][0] = on ? sml[c + w * plan.nchunk][rr][0] : -INFINITY;
+        ml[w][1] = on ? sml[c + w * plan.nchunk][rr][1] : 0.f;
+        mx = fmaxf(mx, ml[w][0]);
       }
-      if (whole) {
-        const int t = (rbase + r) / rep, h = kvh * rep + (rbase + r) % rep;
-        const size_t row = (static_cast<size_t>(b) * p.seq.T + t) * p.Hq + h;
-        const float inv = sum == 0.f ? 0.f : vs / sum;
-        uint2 w;
-        w.x = pt_pack<false>(acc.x * inv, acc.y * inv);
-        w.y = pt_pack<false>(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(p.out + row * D + d) = w;
-        if (d == 0 && p.lse) p.lse[row] = (mx + log2f(sum)) * 0.6931471805599453f;
-      } else {
-        *reinterpret_cast<float4*>(plan.o + (piece * plan.rows + r) * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(plan.ml + (piece * plan.rows + r) * 2) = make_float2(mx, sum);
+#pragma unroll
+      for (int w = 0; w < kPtWarps; ++w) {
+        ml[w][0] = ml[w][0] == mx ? 1.f : pt_exp2(ml[w][0] - mx);
+        sum = fmaf(ml[w][0], ml[w][1], sum);
+      }
+      const float inv = sum == 0.f ? 0.f : vs / sum;
+      const int t = (rbase + r) / rep, h = kvh * rep + (rbase + r) % rep;
+      const size_t row = (static_cast<size_t>(b) * p.seq.T + t) * p.Hq + h;
+#pragma unroll
+      for (int d = 4 * lane; d < D; d += 128) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kPtWarps; ++w)
+          if (w < slots) {
+            const float4 x = *reinterpret_cast<const float4*>(pt_smem + (c + w * plan.nchunk) * S::kWarpBytes +
+                                                              (rr * S::kORow + d) * 4);
+            acc.x = fmaf(ml[w][0], x.x, acc.x);
+            acc.y = fmaf(ml[w][0], x.y, acc.y);
+            acc.z = fmaf(ml[w][0], x.z, acc.z);
+            acc.w = fmaf(ml[w][0], x.w, acc.w);
+          }
+        if (whole)
+          *reinterpret_cast<uint2*>(p.out + row * D + d) =
+              make_uint2(pt_pack<false>(acc.x * inv, acc.y * inv), pt_pack<false>(acc.z * inv, acc.w * inv));
+        else
+          *reinterpret_cast<float4*>(plan.o + (piece * plan.rows + r) * D + d) = acc;
+      }
+      if (lane == 0) {
+        if (!whole) *reinterpret_cast<float2*>(plan.ml + (piece * plan.rows + r) * 2) = make_float2(mx, sum);
+        else if (p.lse) p.lse[row] = (mx + log2f(sum)) * 0.6931471805599453f;
       }
     }
     const int done = t1 - t0;
@@ -578,6 +752,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
       ++b;
       off = 0;
     }
+    if (*static_cast<volatile int*>(&gave_up)) break;  // the results are void; the error word says so
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.seq.err, kErrBitBadInput);
 }
@@ -598,7 +773,7 @@ __global__ void __launch_bounds__(kPtThreads)
             b = static_cast<int>(row / p.Hq / p.seq.T);
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const PagedSpan sp = paged_span(p, b);
+  const PagedSpan sp = paged_span(p, b, plan.tile);
   if (t >= sp.cnt) {  // padding
     for (int d = tid; d < D / 8; d += kPtThreads)
       reinterpret_cast<uint4*>(p.out + row * D)[d] = make_uint4(0u, 0u, 0u, 0u);
@@ -606,14 +781,12 @@ __global__ void __launch_bounds__(kPtThreads)
     return;
   }
   const int kvh = h / rep, r = t * rep + h % rep, item = kvh * plan.groups + r / plan.rows, rr = r % plan.rows;
-  const long long total = __ldcg(plan.pre + p.seq.B);
-  const long long parts = min(static_cast<long long>(plan.ctas), total);
+  const PtLine line(__ldcg(plan.pre + p.seq.B), plan.ctas);
   const long long beg = __ldcg(plan.pre + b) + static_cast<long long>(item) * sp.tiles, end = beg + sp.tiles;
-  // the CTA that holds tile u: the last i with i * total / parts <= u
-  const int first = static_cast<int>(((beg + 1) * parts - 1) / total), last = static_cast<int>((end * parts - 1) / total);
+  const int first = line.owner(beg), last = line.owner(end - 1);
   if (first == last) return;  // one CTA had the whole item
   const auto piece = [&](int i) {  // where CTA i put this item: in its first piece unless it began another before
-    return 2 * static_cast<size_t>(i) + (i * total / parts < beg);
+    return 2 * static_cast<size_t>(i) + (line.start(i) < beg);
   };
   float m = -INFINITY, l = 0.f, acc[kPer];
 #pragma unroll
@@ -680,39 +853,85 @@ __global__ void __launch_bounds__(kPtThreads)
 // ---------------------------------------------------------------------------------------------
 namespace {
 
-// 8-row blocks one warp may hold: as many as leave room for a block of keys and values in registers.
-int pt_max_blocks(int D, bool f8) { return D <= 128 ? 4 : f8 ? 2 : 1; }
-
 struct PtChoice {
-  int nb, nchunk, groups, rows, ctas_per_sm;
+  int nb, nchunk, groups, rows, tile, ctas_per_sm;
 };
 
-PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8) {
-  const int blocks = (T * (Hq / Hkv) + 7) / 8, most = pt_max_blocks(D, f8);
-  PtChoice c;
-  c.nb = blocks >= 3 ? std::min(4, most) : std::min(blocks, most);
-  const int chunks = (blocks + c.nb - 1) / c.nb;
+template <int D, int NB, bool F8>
+PtChoice pt_sizes() {
+  using S = PtShape<D, NB, F8>;
+  return {NB, 1, 1, 8 * NB, kPtWarps * S::kKeys, S::kCtas};
+}
+
+// As many 8-row blocks per warp as there are, up to what the registers hold; then one chunk of rows
+// per warp (the chunks read the same keys), then several row groups.
+template <int D, bool F8>
+PtChoice pt_choose(int T, int Hq, int Hkv) {
+  constexpr int most = PtShape<D, 1, F8>::kMaxNB;
+  const int blocks = (T * (Hq / Hkv) + 7) / 8;
+  const int nb = std::min(most, blocks >= 3 ? 4 : blocks);
+  PtChoice c = nb == 4 ? pt_sizes<D, 4, F8>() : nb == 2 ? pt_sizes<D, 2, F8>() : pt_sizes<D, 1, F8>();
+  const int chunks = (blocks + nb - 1) / nb;
   c.nchunk = chunks >= 3 ? 4 : chunks;
   c.groups = (chunks + c.nchunk - 1) / c.nchunk;
-  c.rows = 8 * c.nb * c.nchunk;
-  c.ctas_per_sm = c.nb * D <= 128 ? 3 : 2;
+  c.rows = 8 * nb * c.nchunk;
   return c;
+}
+
+PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8) {
+  if (D == 64) return f8 ? pt_choose<64, true>(T, Hq, Hkv) : pt_choose<64, false>(T, Hq, Hkv);
+  if (D == 128) return f8 ? pt_choose<128, true>(T, Hq, Hkv) : pt_choose<128, false>(T, Hq, Hkv);
+  return f8 ? pt_choose<256, true>(T, Hq, Hkv) : pt_choose<256, false>(T, Hq, Hkv);
 }
 
 size_t pt_round(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
+// A pool as a matrix of its rows of D elements, to be read in boxes of `box` rows x `line` bytes.  The
+// pages of a pool that interleaves others are further apart: the rows between are never asked for.
+cudaError_t pt_map(CUtensorMap* map, const void* pool, long long page_stride, const PagedAttnParams& p, int es, int line,
+                   int box) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> cached{nullptr};
+  Encode encode = cached.load(std::memory_order_acquire);
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return e;
+    if (!fn || found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    encode = reinterpret_cast<Encode>(fn);
+    cached.store(encode, std::memory_order_release);
+  }
+  const cuuint64_t rows = static_cast<cuuint64_t>(p.seq.n_pages - 1) * (page_stride / p.D) +
+                          static_cast<cuuint64_t>(p.Hkv) * p.seq.page;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.D), rows}, strides[1] = {static_cast<cuuint64_t>(p.D) * es};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(line / es), static_cast<cuuint32_t>(box)}, steps[2] = {1, 1};
+  const CUresult r = encode(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                            const_cast<void*>(pool), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <int D, int NB, bool F8>
 cudaError_t pt_split(const PagedAttnParams& p, const PagedAttnPlan& plan, int dev, cudaLaunchConfig_t cfg) {
+  using S = PtShape<D, NB, F8>;
   static std::atomic<bool> attr_set[64];
   const auto kernel = paged_attn_split_kernel<D, NB, F8>;
-  constexpr int smem = pt_smem_bytes<D, NB, F8>();
+  constexpr int smem = PtShape<D, NB, F8>::kSmem;
   if (!attr_set[dev].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     attr_set[dev].store(true, std::memory_order_release);
   }
+  CUtensorMap kmap, vmap;
+  cudaError_t e = pt_map(&kmap, p.kp, p.kps, p, S::kEs, S::kLine, plan.box);
+  if (e == cudaSuccess) e = pt_map(&vmap, p.vp, p.vps, p, S::kEs, S::kLine, plan.box);
+  if (e != cudaSuccess) return e;
   cfg.dynamicSmemBytes = smem;
-  return cudaLaunchKernelEx(&cfg, kernel, p, plan);
+  return cudaLaunchKernelEx(&cfg, kernel, p, plan, kmap, vmap);
 }
 
 template <int D>
@@ -750,6 +969,12 @@ cudaError_t paged_attn_launch(const PagedAttnParams& p, bool f8, void* ws, int n
   if (dev < 0 || dev >= 64 || n_sm < 1) return cudaErrorInvalidDevice;
   const PtChoice c = pt_choose(p.seq.T, p.Hq, p.Hkv, p.D, f8);
   PagedAttnPlan plan;
+  plan.tile = c.tile;
+  plan.shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.seq.page == 1 << i) plan.shift = i;
+  plan.box = 16;
+  while (p.seq.page % plan.box) plan.box /= 2;
   plan.nchunk = c.nchunk;
   plan.groups = c.groups;
   plan.rows = c.rows;
