@@ -56,18 +56,20 @@ namespace skinny {
 
 constexpr int kPtThreads = 128;
 constexpr int kPtWarps = kPtThreads / 32;
-constexpr uint32_t kPtNone = 0xFFFFFFFFu;  // no such key (past the end, or a page outside the pool)
-constexpr float kPtSlack = 8.f;           // how far p may exceed 1, in powers of two
+constexpr int kPtLead = 2;
+constexpr float kPtMost = 256.f;          // how far p may exceed 1 before the maximum is renewed
+constexpr float kPtNothing = -3.402823466e38f;  // the maximum of a row that has seen no key
 
 struct PagedAttnPlan {
-  int tile;        // keys of one unit of work: one block per warp
+  int tile_log;    // keys of one tile, one block per warp (a power of two)
+  int lead;        // what beginning an item costs, in tiles: counted on the line, so that the pieces balance
   int shift;       // log2 of the page size, or -1
   int box;         // positions of one copy: the largest power of two up to 16 that divides the page size
   int nchunk;      // row chunks of 8 NB rows, one per warp (1, 2 or 4); the other warps split keys
   int groups;      // row groups of nchunk chunks per kv head
   int rows;        // rows of one group: 8 NB nchunk
   int ctas;        // CTAs of the split launch
-  long long* pre;  // [B + 1] first tile of each sequence on the line
+  long long* pre;  // [B + 1] where each sequence begins on the line
   float* ml;       // [2 ctas][rows][2] maximum (log2) and sum of a piece
   float* o;        // [2 ctas][rows][D]
 };
@@ -76,16 +78,19 @@ struct PagedAttnPlan {
 struct PagedSpan {
   int len, cnt, beg, end;
   int first, tiles;  // the tiles start at a multiple of 32: no box straddles two blocks
+  int units;         // tiles and lead of one item on the line
 };
 
-__device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, int b, int tile, bool* ok = nullptr) {
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, const PagedAttnPlan& plan, int b,
+                                                bool* ok = nullptr) {
   PagedSpan s;
   const bool good = p.seq.get(b, s.len, s.cnt);
   if (ok) *ok = good;
   s.end = s.len + s.cnt;
   s.beg = p.window > 0 && s.len >= p.window ? s.len - p.window + 1 : 0;
   s.first = s.beg & ~31;
-  s.tiles = s.cnt > 0 ? (s.end - s.first + tile - 1) / tile : 0;
+  s.tiles = s.cnt > 0 ? ((s.end - s.first - 1) >> plan.tile_log) + 1 : 0;
+  s.units = s.tiles ? s.tiles + plan.lead : 0;
   return s;
 }
 
@@ -138,7 +143,7 @@ __device__ __forceinline__ long long pt_div(long long a, long long b) {
   return a / b;
 }
 
-// The line's pieces: `total` tiles over `parts` CTAs, the first `rest` of them one tile longer.
+// The line's pieces: `total` units over the CTAs, the first `rest` pieces one unit longer.
 struct PtLine {
   long long total, each, rest;
   __device__ __forceinline__ PtLine(long long n, int ctas) : total(n), each(0), rest(0) {
@@ -186,6 +191,8 @@ struct PtShape {
   static constexpr int kCtas = NB * D <= 128 ? 3 : 2;            // CTAs per SM
   static constexpr int kKBytes = kKeys * kRow;                   // keys (or values) of one block
   static constexpr int kStages = 16384 / (2 * kKBytes);
+  static constexpr bool kJoint = kStages > 1;  // keys and values of a block on one barrier (else the one is fetched
+                                               // again while the other is in use)
   static constexpr int kMaxNB = D <= 128 ? 4 : F8 ? 2 : 1;
   static constexpr int kChunks = NB == kMaxNB ? kPtWarps : 1;    // row chunks a CTA may hold
   static constexpr int kORow = D + 4;                            // floats of one row of O in shared memory
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   constexpr int kSub = S::kSub, kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t pt_raw[];
   uint8_t* const pt_smem = pt_raw + ((1024 - (smem_u32(pt_raw) & 1023)) & 1023);  // swizzle periods are 1 KB
-  __shared__ uint64_t bars[kPtWarps][kStages][2];  // per warp and stage: the keys are there, the values are there
+  __shared__ uint64_t bars[kPtWarps][kStages][2];  // per warp and stage: the block (its keys, its values) is there
   __shared__ int gave_up;                          // a wait ran out
   __shared__ float sml[kPtWarps][8 * NB][2];
   __shared__ float sdown[S::kChunks * 8 * NB];  // e4m3: the power of two each row's q was divided by
@@ -212,69 +219,98 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   __shared__ long long found[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cq = lane & 3;
   const int rep = p.Hq / p.Hkv, items = p.Hkv * plan.groups, B = p.seq.B;
+  const uint32_t bar0 = smem_u32(&bars[warp][0][0]);
   pdl_launch_dependents();
-  if (tid < kPtWarps * kStages * 2) mbar_init(smem_u32(&bars[0][0][0]) + 8 * tid, 1);
+  if (lane < kStages * 2) mbar_init(bar0 + 8 * lane, 1);
   if (tid == 0) gave_up = 0;
   fence_mbar_init();
+  __syncthreads();
   pdl_wait_prior_grid();
 
-  // ---- this CTA's piece of the line: thread i sums the tiles of its run of sequences
-  const int run = (B + kPtThreads - 1) / kPtThreads, b_lo = min(B, tid * run), b_hi = min(B, b_lo + run);
-  long long mine = 0;
-  bool all_ok = true;
-  for (int b = b_lo; b < b_hi; ++b) {
-    bool ok;
-    mine += static_cast<long long>(paged_span(p, b, plan.tile, &ok).tiles) * items;
-    all_ok &= ok;
-  }
-  long long incl = mine;
+  // ---- this CTA's piece of the line: [u, u_end), beginning `off` units into sequence b
+  int b;
+  long long u, u_end, off;
+  if (B <= 32) {  // one sequence per lane, every warp by itself
+    bool ok = true;
+    const long long mine =
+        lane < B ? static_cast<long long>(paged_span(p, plan, lane, &ok).units) * items : 0;
+    long long incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if (lane >= o) incl += x;
-  }
-  if (lane == 31) scan[warp] = incl;
-  __syncthreads();
-  long long total = 0, excl = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kPtWarps; ++w) {
-    if (w < warp) excl += scan[w];
-    total += scan[w];
-  }
-  if (blockIdx.x == 0) {  // the join's copy of the line
-    long long at = excl;
-    for (int b = b_lo; b < b_hi; ++b) {
-      plan.pre[b] = at;
-      at += static_cast<long long>(paged_span(p, b, plan.tile).tiles) * items;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += x;
     }
-    if (tid == 0) plan.pre[B] = total;
-    if (!all_ok) atomicOr(p.seq.err, kErrBitBadInput);
-  }
-  if (blockIdx.x >= total) return;
-  const PtLine line(total, plan.ctas);
-  long long u = line.start(blockIdx.x);
-  const long long u_end = line.start(blockIdx.x + 1);
-  if (excl <= u && u < excl + mine) {
-    long long at = excl;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const long long n = static_cast<long long>(paged_span(p, b, plan.tile).tiles) * items;
-      if (u < at + n) {
-        found[0] = b;
-        found[1] = u - at;
-        break;
+    const long long total = __shfl_sync(0xFFFFFFFFu, incl, 31);
+    if (blockIdx.x == 0 && warp == 0) {
+      if (lane < B) plan.pre[lane] = incl - mine;  // the join's copy of the line
+      if (lane == 0) plan.pre[B] = total;
+      if (!ok) atomicOr(p.seq.err, kErrBitBadInput);
+    }
+    if (blockIdx.x >= total) return;
+    const PtLine line(total, plan.ctas);
+    u = line.start(blockIdx.x);
+    u_end = line.start(blockIdx.x + 1);
+    b = __ffs(__ballot_sync(0xFFFFFFFFu, u < incl)) - 1;
+    off = u - __shfl_sync(0xFFFFFFFFu, incl - mine, b);
+  } else {  // thread i sums its run of sequences
+    const int run = (B + kPtThreads - 1) / kPtThreads, b_lo = min(B, tid * run), b_hi = min(B, b_lo + run);
+    long long mine = 0;
+    bool all_ok = true;
+    for (int i = b_lo; i < b_hi; ++i) {
+      bool ok;
+      mine += static_cast<long long>(paged_span(p, plan, i, &ok).units) * items;
+      all_ok &= ok;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    long long total = 0, excl = incl - mine;
+#pragma unroll
+    for (int w = 0; w < kPtWarps; ++w) {
+      if (w < warp) excl += scan[w];
+      total += scan[w];
+    }
+    if (blockIdx.x == 0) {
+      long long at = excl;
+      for (int i = b_lo; i < b_hi; ++i) {
+        plan.pre[i] = at;
+        at += static_cast<long long>(paged_span(p, plan, i).units) * items;
       }
-      at += n;
+      if (tid == 0) plan.pre[B] = total;
+      if (!all_ok) atomicOr(p.seq.err, kErrBitBadInput);
     }
+    if (blockIdx.x >= total) return;
+    const PtLine line(total, plan.ctas);
+    u = line.start(blockIdx.x);
+    u_end = line.start(blockIdx.x + 1);
+    if (excl <= u && u < excl + mine) {
+      long long at = excl;
+      for (int i = b_lo; i < b_hi; ++i) {
+        const long long n = static_cast<long long>(paged_span(p, plan, i).units) * items;
+        if (u < at + n) {
+          found[0] = i;
+          found[1] = u - at;
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+    b = static_cast<int>(found[0]);
+    off = found[1];
   }
-  __syncthreads();
-  int b = static_cast<int>(found[0]);
-  long long off = found[1];
+
   const int chunk = warp % plan.nchunk, slot = warp / plan.nchunk, slots = kPtWarps / plan.nchunk;
   const uint32_t kpr = static_cast<uint32_t>(p.kps / D), vpr = static_cast<uint32_t>(p.vps / D);
+  const int boxes = S::kKeys / plan.box, boxes_log = __ffs(boxes) - 1;  // copies of one line of a block
   uint8_t* const region = pt_smem + warp * S::kWarpBytes;
   float* const so = reinterpret_cast<float*>(region);                  // [8 NB][kORow], after the loop
   const uint32_t ring = smem_u32(region);                               // [stage][keys | values][line][key][kLine], swizzled
-  const uint32_t bar0 = smem_u32(&bars[warp][0][0]);
   // Fragment addresses inside a block.  Swizzle: 16-byte piece c of a 128-byte line of key k lies at
   // c ^ (k & 7), of a 64-byte line at c ^ (k / 2 & 3).  K by ldmatrix: lanes 0-15 keys 0-15 at piece 2 i,
   // lanes 16-31 at 2 i + 1 (the piece's step is an xor).  V: keys 2 cq + (e & 1) + 8 (e >> 1), dims from 8 g
@@ -289,19 +325,41 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   uint32_t pending = 0, parity = 0;    // per barrier (bit 2 stage + what): copies in flight, the phase they complete
   bool bad = false;
 
-  for (int seg = 0; u < u_end; ++seg) {
-    const PagedSpan sp = paged_span(p, b, plan.tile);
+  for (int seg = 0; u < u_end;) {
+    const PagedSpan sp = paged_span(p, plan, b);
     if (sp.tiles == 0) {
       ++b;
-      --seg;
       continue;
     }
-    const int item = static_cast<int>(pt_div(off, sp.tiles)), t0 = static_cast<int>(off - static_cast<long long>(item) * sp.tiles);
-    const int t1 = static_cast<int>(min(static_cast<long long>(sp.tiles), t0 + (u_end - u)));
+    const int item = static_cast<int>(pt_div(off, sp.units)), at = static_cast<int>(off - static_cast<long long>(item) * sp.units);
+    const int take = static_cast<int>(min(static_cast<long long>(sp.units - at), u_end - u));
+    const int t0 = max(at - plan.lead, 0), t1 = max(at + take - plan.lead, 0), cur = b;
+    u += take;
+    off += take;
+    if (off == static_cast<long long>(sp.units) * items) {
+      ++b;
+      off = 0;
+    }
+    if (t1 <= t0) continue;  // only an item's lead
     const int kvh = item / plan.groups, rbase = (item % plan.groups) * plan.rows;
-    const int k0 = sp.first + t0 * plan.tile, k1 = min(sp.end, sp.first + t1 * plan.tile);
+    const int k0 = sp.first + (t0 << plan.tile_log), k1 = min(sp.end, sp.first + (t1 << plan.tile_log));
     const int r0 = rbase + chunk * 8 * NB;  // this warp's first row
-    const int32_t* const table = p.seq.table + b * p.seq.table_stride;
+    const int32_t* const table = p.seq.table + cur * p.seq.table_stride;
+
+    // ---- the query rows, 8 dims per thread at a time: asked for before the keys and values
+    constexpr int kQBatch = NB * D / 128 < 1 ? 1 : NB * D / 128;  // pieces per thread of one chunk
+    const auto q_load = [&](int e) {
+      const int r = rbase + e / (D / 8), t = r / rep, h = kvh * rep + (r - t * rep);
+      return t < sp.cnt ? __ldg(reinterpret_cast<const uint4*>(p.q + cur * p.qs[0] + t * p.qs[1] + h * p.qs[2]) + e % (D / 8))
+                        : make_uint4(0u, 0u, 0u, 0u);
+    };
+    const int q_pieces = plan.rows * (D / 8);
+    uint4 qw[kQBatch];
+#pragma unroll
+    for (int i = 0; i < kQBatch; ++i) {
+      const int e = tid + i * kPtThreads;
+      if (e < q_pieces) qw[i] = q_load(e);
+    }
 
     // ---- this warp's blocks of keys: block n holds the keys from k0 + kKeys (n slots + slot)
     const int nblk_all = (k1 - k0 + S::kKeys - 1) / S::kKeys;
@@ -319,37 +377,42 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     const auto rows_of = [&](int pid, int in_page) {  // -> the keys that exist, one bit each
       const bool ok = pid >= 0 && pid < p.seq.n_pages;
       bad |= !ok && pid != -2;
-      const uint32_t at = static_cast<uint32_t>(kvh) * p.seq.page + static_cast<uint32_t>(in_page);
-      rk = ok ? static_cast<uint32_t>(pid) * kpr + at : kPtNone;
-      rv = ok ? static_cast<uint32_t>(pid) * vpr + at : kPtNone;
+      const uint32_t in = static_cast<uint32_t>(kvh) * p.seq.page + static_cast<uint32_t>(in_page);
+      rk = static_cast<uint32_t>(pid) * kpr + in;
+      rv = static_cast<uint32_t>(pid) * vpr + in;
       return __ballot_sync(0xFFFFFFFFu, ok);
     };
-    // The block whose pages were looked up last (one key per lane) into stage st, one box per lane; its
-    // slots have been read by all lanes.  A box without a key that exists is left out.
-    const auto copy = [&](int st, int what, uint32_t r, uint32_t exist) {
-      const uint32_t bar = bar0 + (st * 2 + what) * 8;
-      const int first = lane * plan.box;
-      const uint32_t here = first < S::kKeys ? exist & ((1u << plan.box) - 1u) << first : 0u;
-      const int src = here ? __ffs(here) - 1 : 0;
-      const uint32_t row = __shfl_sync(0xFFFFFFFFu, r, src) - static_cast<uint32_t>(src - first);
-      const int boxes = __popc(__ballot_sync(0xFFFFFFFFu, here != 0));
-      if (lane == 0) mbar_arrive_expect_tx(bar, boxes * plan.box * S::kRow);
+    // The block whose pages were looked up last (one key per lane) into stage st, one copy per lane; its
+    // slots have been read by all lanes.  what: 0 keys, 1 values, 2 both (on the keys' barrier).  A box
+    // without a key that exists is left out.
+    const auto copy = [&](int st, int what, uint32_t exist) {
+      const int bit = st * 2 + (what & 1);
+      const uint32_t bar = bar0 + bit * 8;
+      const uint32_t mask = (1u << plan.box) - 1u;
+      const int some = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && (exist >> (lane * plan.box) & mask)));
+      if (lane == 0) mbar_arrive_expect_tx(bar, some * plan.box * S::kRow * (what == 2 ? 2 : 1));
       __syncwarp();
-      if (here) {
-        const uint32_t dst = ring + (st * 2 + what) * S::kKBytes + first * S::kLine;
-        if (S::kLine == 64 && plan.box == 1) {  // 64 bytes: less than a tiled copy's alignment
-          const uint8_t* const from = static_cast<const uint8_t*>(what ? p.vp : p.kp) + static_cast<size_t>(row) * S::kRow;
-          for (int c = 0; c < 4; ++c) bulk_g2s(dst + ((c ^ (first >> 1 & 3)) << 4), from + 16 * c, 16, bar);
-        } else {
-#pragma unroll
-          for (int c = 0; c < S::kLines; ++c)
-            tma_load_2d(dst + c * (S::kKeys * S::kLine), what ? &vmap : &kmap, c * (S::kLine / S::kEs), static_cast<int>(row), bar);
+      const int n = (boxes << (what == 2 ? 1 : 0)) * S::kLines;
+      for (int q0 = 0; q0 < n; q0 += 32) {
+        const int q = q0 + lane, first = (q & (boxes - 1)) * plan.box, rest = q >> boxes_log;
+        const int kv = what == 2 ? rest & 1 : what, line = what == 2 ? rest >> 1 : rest;
+        const uint32_t here = exist & mask << first;
+        const int src = here ? __ffs(here) - 1 : 0;
+        const uint32_t row_k = __shfl_sync(0xFFFFFFFFu, rk, src), row_v = __shfl_sync(0xFFFFFFFFu, rv, src);
+        const uint32_t row = (kv ? row_v : row_k) - static_cast<uint32_t>(src - first);
+        if (q < n && here) {
+          const uint32_t dst = ring + (st * 2 + kv) * S::kKBytes + (line * S::kKeys + first) * S::kLine;
+          if (S::kLine == 64 && plan.box == 1) {  // 64 bytes: less than a tiled copy's alignment
+            const uint8_t* const from = static_cast<const uint8_t*>(kv ? p.vp : p.kp) + static_cast<size_t>(row) * S::kRow;
+            for (int c = 0; c < 4; ++c) bulk_g2s(dst + ((c ^ (first >> 1 & 3)) << 4), from + 16 * c, 16, bar);
+          } else {
+            tma_load_2d(dst, kv ? &vmap : &kmap, line * (S::kLine / S::kEs), static_cast<int>(row), bar);
+          }
         }
       }
-      pending |= 1u << (st * 2 + what);
+      pending |= 1u << bit;
     };
-    const auto arrived = [&](int st, int what) {  // bounded; the same answer in every lane
-      const int bit = st * 2 + what;
+    const auto arrived = [&](int bit) {  // bounded; the same answer in every lane
       const bool ok = mbar_wait(bar0 + bit * 8, parity >> bit & 1u, p.seq.err, kErrBitWaitFull, &gave_up);
       if (!__all_sync(0xFFFFFFFFu, ok)) return false;
       pending &= ~(1u << bit);
@@ -366,26 +429,29 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
         pid[st] = page_of(st, in[st]);
       }
       pid_next = page_of(kStages, in_next);
-      fence_proxy_async_smem();  // the previous segment's O was written here by ordinary stores
-      __syncthreads();           // and has been read
+      if (seg > 0) {
+        fence_proxy_async_smem();  // the previous segment's O was written here by ordinary stores
+        __syncthreads();           // and has been read
+      }
 #pragma unroll
       for (int st = 0; st < kStages; ++st) {
         have[st] = rows_of(pid[st], in[st]);
         if (st < nblk) {
-          const int at = stage + st < kStages ? stage + st : stage + st - kStages;
-          copy(at, 0, rk, have[st]);
-          copy(at, 1, rv, have[st]);
+          const int where = stage + st < kStages ? stage + st : stage + st - kStages;
+          if (S::kJoint) {
+            copy(where, 2, have[st]);
+          } else {
+            copy(where, 0, have[st]);
+            copy(where, 1, have[st]);
+          }
         }
       }
     }
 
-    // ---- the query rows to shared memory, 8 dims per thread at a time
+    // ---- the query rows to shared memory
     const float sc0 = p.scale * 1.4426950408889634f * (F8 ? p.k_scale[kvh] : 1.f);
-    for (int e = tid; e < plan.rows * (D / 8); e += kPtThreads) {
+    const auto q_store = [&](int e, uint4 w) {
       const int row = e / (D / 8), u8 = e % (D / 8);
-      const int r = rbase + row, t = r / rep, h = kvh * rep + r % rep;
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (t < sp.cnt) w = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs[0] + t * p.qs[1] + h * p.qs[2]) + u8);
       uint8_t* const dst = sq + row * S::kQPad;
       if (F8) {  // to f16, the row's largest |q| to [1, 2); pairs 0, 2, .. of 16 dims before pairs 1, 3, ..
         uint32_t x[4] = {w.x, w.y, w.z, w.w}, top = 0;
@@ -403,7 +469,13 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
       } else {
         reinterpret_cast<uint4*>(dst)[u8] = w;
       }
+    };
+#pragma unroll
+    for (int i = 0; i < kQBatch; ++i) {
+      const int e = tid + i * kPtThreads;
+      if (e < q_pieces) q_store(e, qw[i]);
     }
+    for (int e = tid + kQBatch * kPtThreads; e < q_pieces; e += kPtThreads) q_store(e, q_load(e));
     __syncthreads();
     // fragments by ldmatrix: rows 0-7 of a block at 16-byte pieces 4 i .. 4 i + 3
     const uint32_t qaddr = smem_u32(sq) + (chunk * 8 * NB + (lane & 7)) * S::kQPad + (lane >> 3) * 16;
@@ -429,20 +501,26 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     } else {
       sc[0][0] = sc[0][1] = sc0;
     }
+    // the tokens of this lane's rows, 4 bits each (rows past the last token: any)
+    uint32_t tokens = 0;
+    if (p.seq.T > 1) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) tokens |= min(15, (r0 + 8 * (i >> 1) + 2 * cq + (i & 1)) / rep) << (4 * i);
+    }
 
     // ---- one pass over the blocks
     float o[NB][S::kTiles][4], m[NB][2], l[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      m[nb][0] = m[nb][1] = -INFINITY;
+      m[nb][0] = m[nb][1] = kPtNothing;
       l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < S::kTiles; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nb][i][e] = 0.f;
     }
-    const auto sees = [&](int row, int j) {  // does row r0 + row see position j
-      const int pos = sp.len + (r0 + row) / rep;
+    const auto sees = [&](int t, int j) {  // does token t see position j
+      const int pos = sp.len + t;
       return j <= pos && (p.window <= 0 || j > pos - p.window);
     };
     const auto is_edge = [&](int j0) {  // a block that some row sees only part of
@@ -462,7 +540,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int sub = 0; sub < kSub; ++sub) s[nb][sub][0] = s[nb][sub][1] = s[nb][sub][2] = s[nb][sub][3] = 0.f;
-      if (!arrived(stage, 0)) break;
+      if (!arrived(stage * 2)) break;
 #pragma unroll
       for (int i = 0; i < S::kRow / 32; ++i) {  // 32 bytes of 16 (32) keys: one 16-dim step, or two of e4m3
         uint32_t kw[kSub][4];
@@ -507,40 +585,56 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
           }
         }
       }
-      if (n + kStages < nblk) copy(stage, 0, rk, have_next);
+      if (!S::kJoint && n + kStages < nblk) copy(stage, 0, have_next);
       constexpr uint32_t kAll = 0xFFFFFFFFu;
-      const bool edge = is_edge(j0) || now != kAll;
-      bool up = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = -INFINITY;
+        for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nb][sub][e] *= sc[F8 ? nb : 0][e & 1];
+      if (is_edge(j0) || now != kAll) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int t = tokens >> (4 * (2 * nb + e)) & 15u;
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                const int key = 16 * sub + 8 * hf + g;
+                if (!(now >> key & 1u) || !sees(t, j0 + key)) s[nb][sub][2 * hf + e] = -INFINITY;
+              }
+          }
+      }
+      // p = 2^(s - m), with the maximum of the blocks before
+      float pr[NB][kSub][4];
+      const auto exponentials = [&]() {
+        float top = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int sub = 0; sub < kSub; ++sub)
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              float& x = s[nb][sub][2 * hf + e];
-              x *= sc[F8 ? nb : 0][e];
-              if (edge) {
-                const int key = 16 * sub + 8 * hf + g;
-                if (!(now >> key & 1u) || !sees(8 * nb + 2 * cq + e, j0 + key)) x = -INFINITY;
-              }
-              top = fmaxf(top, x);
+            for (int e = 0; e < 4; ++e) {
+              pr[nb][sub][e] = pt_exp2(s[nb][sub][e] - m[nb][e & 1]);
+              top = fmaxf(top, pr[nb][sub][e]);
             }
-          up |= top > m[nb][e] + kPtSlack;
-        }
-      if (__any_sync(0xFFFFFFFFu, up)) {  // renew the maxima, rescale the sums
+        return top;
+      };
+      if (__any_sync(0xFFFFFFFFu, exponentials() > kPtMost)) {  // renew the maxima, rescale the sums
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float x = m[nb][e];
 #pragma unroll
-            for (int sub = 0; sub < kSub; ++sub) x = fmaxf(x, fmaxf(s[nb][sub][e], s[nb][sub][2 + e]));
+            for (int sub = 0; sub < kSub; ++sub)
+              x = fmaxf(x, fmaxf(s[nb][sub][e], s[nb][sub][2 + e]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, w));
-            const float f = m[nb][e] == x ? 1.f : pt_exp2(m[nb][e] - x);
+            const float f = pt_exp2(m[nb][e] - x);
             m[nb][e] = x;
             l[nb][e] *= f;
 #pragma unroll
@@ -549,25 +643,20 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
               o[nb][q][2 + e] *= f;
             }
           }
+        exponentials();
       }
       uint32_t pb[NB][kSub][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int sub = 0; sub < kSub; ++sub) {
-          float(&x)[4] = s[nb][sub];
-          x[0] = pt_exp2(x[0] - m0);
-          x[1] = pt_exp2(x[1] - m1);
-          x[2] = pt_exp2(x[2] - m0);
-          x[3] = pt_exp2(x[3] - m1);
+          const float(&x)[4] = pr[nb][sub];
           l[nb][0] += x[0] + x[2];
           l[nb][1] += x[1] + x[3];
           pb[nb][sub][0] = pt_transpose(pt_pack<F8>(x[0], x[1]));
           pb[nb][sub][1] = pt_transpose(pt_pack<F8>(x[2], x[3]));
         }
-      }
-      if (!arrived(stage, 1)) break;
+      if (!S::kJoint && !arrived(stage * 2 + 1)) break;
       if (now != kAll) {  // keys that do not exist multiply zeros
         if (lane < S::kKeys && !(now >> lane & 1u))
 #pragma unroll
@@ -635,22 +724,22 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
             }
           }
         }
-      if (n + kStages < nblk) copy(stage, 1, rv, have_next);
+      if (n + kStages < nblk) copy(stage, S::kJoint ? 2 : 1, have_next);
 #pragma unroll
       for (int st = 0; st + 1 < kStages; ++st) have[st] = have[st + 1];
       have[kStages - 1] = have_next;
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
     if (pending) {  // gave up: no copy may land after the CTA has left (bounded again)
-      const uint64_t t0 = globaltimer_ns();
+      const uint64_t since = globaltimer_ns();
       for (int bit = 0; bit < 2 * kStages; ++bit)
         while ((pending >> bit & 1u) && !mbar_try_wait(bar0 + bit * 8, parity >> bit & 1u) &&
-               globaltimer_ns() - t0 < SKINNY_WAIT_NS) {
+               globaltimer_ns() - since < SKINNY_WAIT_NS) {
         }
     }
 
     // ---- the warps' results: (maximum, sum) and O to shared memory, joined row by row
-    __syncwarp();  // the ring's slots of all lanes are free
+    __syncwarp();  // the ring's slots have been read
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -678,22 +767,22 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
 #pragma unroll 1
         for (int j = j0; is_edge(j0) && j < min(j0 + S::kKeys, k1); ++j) {
           const int pid = table[j / p.seq.page];
-          if (pid < 0 || pid >= p.seq.n_pages) continue;
-          const size_t at = pid * static_cast<size_t>(p.vps) + (static_cast<size_t>(kvh) * p.seq.page + j % p.seq.page) * D;
+          if (j < sp.beg || pid < 0 || pid >= p.seq.n_pages) continue;
+          const size_t where = pid * static_cast<size_t>(p.vps) + (static_cast<size_t>(kvh) * p.seq.page + j % p.seq.page) * D;
 #pragma unroll 1
           for (int d = lane; d < D; d += 32) {
             float v;
             if (F8) {
               __nv_fp8_e4m3 x;
-              x.__x = static_cast<const uint8_t*>(p.vp)[at + d];
+              x.__x = static_cast<const uint8_t*>(p.vp)[where + d];
               v = static_cast<float>(x);
             } else {
-              v = __bfloat162float(static_cast<const __nv_bfloat16*>(p.vp)[at + d]);
+              v = __bfloat162float(static_cast<const __nv_bfloat16*>(p.vp)[where + d]);
             }
             if (!isfinite(v))
 #pragma unroll 1
               for (int r = 0; r < 8 * NB; ++r)
-                if (sees(r, j)) so[r * S::kORow + d] += v;
+                if (sees((r0 + r) / rep, j)) so[r * S::kORow + d] += v;
           }
         }
       }
@@ -701,26 +790,40 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     __syncthreads();
     const bool whole = t0 == 0 && t1 == sp.tiles;
     const size_t piece = 2 * static_cast<size_t>(blockIdx.x) + (seg > 0);
-    const float vs = F8 ? p.v_scale[kvh] : 1.f;
     const int live = min(plan.rows, sp.cnt * rep - rbase);  // rows of the group that exist
-    for (int r = warp; r < live; r += kPtWarps) {
-      const int c = r / (8 * NB), rr = r % (8 * NB);
-      float ml[kPtWarps][2], mx = -INFINITY, sum = 0.f;  // over the warps of the row's chunk
+    // warp w finishes rows w, w + 4, ...: lane i first works out the weights of row w + 4 i
+    float f[kPtWarps], inv = 0.f;
+    int out_row = 0;
+    {
+      const int r = min(warp + kPtWarps * lane, plan.rows - 1), c = r / (8 * NB), rr = r % (8 * NB);
+      float mx = kPtNothing, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPtWarps; ++w)
+        if (w < slots) mx = fmaxf(mx, sml[c + w * plan.nchunk][rr][0]);
 #pragma unroll
       for (int w = 0; w < kPtWarps; ++w) {
-        const bool on = w < slots;
-        ml[w][0] = on ? sml[c + w * plan.nchunk][rr][0] : -INFINITY;
-        ml[w][1] = on ? sml[c + w * plan.nchunk][rr][1] : 0.f;
-        mx = fmaxf(mx, ml[w][0]);
+        f[w] = 0.f;
+        if (w < slots) {
+          f[w] = pt_exp2(sml[c + w * plan.nchunk][rr][0] - mx);
+          sum = fmaf(f[w], sml[c + w * plan.nchunk][rr][1], sum);
+        }
       }
+      const int t = (rbase + r) / rep, h = kvh * rep + (rbase + r - t * rep);
+      out_row = (cur * p.seq.T + t) * p.Hq + h;
+      inv = sum == 0.f ? 0.f : (F8 ? p.v_scale[kvh] : 1.f) / sum;
+      if (warp + kPtWarps * lane < live) {
+        if (!whole) *reinterpret_cast<float2*>(plan.ml + (piece * plan.rows + r) * 2) = make_float2(mx, sum);
+        else if (p.lse) p.lse[out_row] = (mx + log2f(sum)) * 0.6931471805599453f;
+      }
+    }
+#pragma unroll 2
+    for (int i = 0; warp + kPtWarps * i < live; ++i) {
+      const int r = warp + kPtWarps * i, c = r / (8 * NB), rr = r % (8 * NB);
+      float fr[kPtWarps];
 #pragma unroll
-      for (int w = 0; w < kPtWarps; ++w) {
-        ml[w][0] = ml[w][0] == mx ? 1.f : pt_exp2(ml[w][0] - mx);
-        sum = fmaf(ml[w][0], ml[w][1], sum);
-      }
-      const float inv = sum == 0.f ? 0.f : vs / sum;
-      const int t = (rbase + r) / rep, h = kvh * rep + (rbase + r) % rep;
-      const size_t row = (static_cast<size_t>(b) * p.seq.T + t) * p.Hq + h;
+      for (int w = 0; w < kPtWarps; ++w) fr[w] = __shfl_sync(0xFFFFFFFFu, f[w], i);
+      const float iv = __shfl_sync(0xFFFFFFFFu, inv, i);
+      const size_t row = __shfl_sync(0xFFFFFFFFu, out_row, i);
 #pragma unroll
       for (int d = 4 * lane; d < D; d += 128) {
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -729,96 +832,89 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
           if (w < slots) {
             const float4 x = *reinterpret_cast<const float4*>(pt_smem + (c + w * plan.nchunk) * S::kWarpBytes +
                                                               (rr * S::kORow + d) * 4);
-            acc.x = fmaf(ml[w][0], x.x, acc.x);
-            acc.y = fmaf(ml[w][0], x.y, acc.y);
-            acc.z = fmaf(ml[w][0], x.z, acc.z);
-            acc.w = fmaf(ml[w][0], x.w, acc.w);
+            acc.x = fmaf(fr[w], x.x, acc.x);
+            acc.y = fmaf(fr[w], x.y, acc.y);
+            acc.z = fmaf(fr[w], x.z, acc.z);
+            acc.w = fmaf(fr[w], x.w, acc.w);
           }
         if (whole)
           *reinterpret_cast<uint2*>(p.out + row * D + d) =
-              make_uint2(pt_pack<false>(acc.x * inv, acc.y * inv), pt_pack<false>(acc.z * inv, acc.w * inv));
+              make_uint2(pt_pack<false>(acc.x * iv, acc.y * iv), pt_pack<false>(acc.z * iv, acc.w * iv));
         else
           *reinterpret_cast<float4*>(plan.o + (piece * plan.rows + r) * D + d) = acc;
       }
-      if (lane == 0) {
-        if (!whole) *reinterpret_cast<float2*>(plan.ml + (piece * plan.rows + r) * 2) = make_float2(mx, sum);
-        else if (p.lse) p.lse[row] = (mx + log2f(sum)) * 0.6931471805599453f;
-      }
     }
-    const int done = t1 - t0;
-    u += done;
-    off += done;
-    if (off == static_cast<long long>(sp.tiles) * items) {
-      ++b;
-      off = 0;
-    }
+    ++seg;
     if (*static_cast<volatile int*>(&gave_up)) break;  // the results are void; the error word says so
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.seq.err, kErrBitBadInput);
 }
 
 // Joins the pieces of the items that were split, one output row per CTA, and writes the rows that no
-// piece covers (idle slots, padding).  Warp w adds pieces w, w + 4, ... and the four results are
-// added in order.
+// piece covers (idle slots, padding).  Warp w adds pieces w, w + 8, ... and the results are added in
+// order.
+constexpr int kPtJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(kPtThreads)
+__global__ void __launch_bounds__(32 * kPtJoinWarps)
     paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ PagedAttnPlan plan) {
   constexpr int kPer = D / 32;
   constexpr int kAhead = 4;  // pieces whose loads are issued together
-  __shared__ float so[kPtWarps][D], sml[kPtWarps][2];
+  __shared__ float so[kPtJoinWarps][D], sml[kPtJoinWarps][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rep = p.Hq / p.Hkv;
-  const size_t row = blockIdx.x;
-  const int h = static_cast<int>(row % p.Hq), t = static_cast<int>(row / p.Hq % p.seq.T),
-            b = static_cast<int>(row / p.Hq / p.seq.T);
+  const int row = blockIdx.x, bt = row / p.Hq, h = row - bt * p.Hq, b = bt / p.seq.T, t = bt - b * p.seq.T;
+  const int kvh = h / rep, r = t * rep + (h - kvh * rep), group = r / plan.rows, rr = r - group * plan.rows;
+  const int item = kvh * plan.groups + group;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const PagedSpan sp = paged_span(p, b, plan.tile);
+  const long long begins = __ldcg(plan.pre + b), total = __ldcg(plan.pre + p.seq.B);
+  const PagedSpan sp = paged_span(p, plan, b);
   if (t >= sp.cnt) {  // padding
-    for (int d = tid; d < D / 8; d += kPtThreads)
-      reinterpret_cast<uint4*>(p.out + row * D)[d] = make_uint4(0u, 0u, 0u, 0u);
+    if (tid < D / 8) reinterpret_cast<uint4*>(p.out + static_cast<size_t>(row) * D)[tid] = make_uint4(0u, 0u, 0u, 0u);
     if (tid == 0 && p.lse) p.lse[row] = -INFINITY;
     return;
   }
-  const int kvh = h / rep, r = t * rep + h % rep, item = kvh * plan.groups + r / plan.rows, rr = r % plan.rows;
-  const PtLine line(__ldcg(plan.pre + p.seq.B), plan.ctas);
-  const long long beg = __ldcg(plan.pre + b) + static_cast<long long>(item) * sp.tiles, end = beg + sp.tiles;
-  const int first = line.owner(beg), last = line.owner(end - 1);
+  const PtLine line(total, plan.ctas);
+  const long long beg = begins + static_cast<long long>(item) * sp.units;
+  const int first = line.owner(beg + plan.lead), last = line.owner(beg + sp.units - 1);
   if (first == last) return;  // one CTA had the whole item
   const auto piece = [&](int i) {  // where CTA i put this item: in its first piece unless it began another before
     return 2 * static_cast<size_t>(i) + (line.start(i) < beg);
   };
-  float m = -INFINITY, l = 0.f, acc[kPer];
+  float m = kPtNothing, l = 0.f, acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int i0 = first + warp; i0 <= last; i0 += kPtWarps * kAhead) {
+  for (int i0 = first + warp; i0 <= last; i0 += kPtJoinWarps * kAhead) {
     float2 ml[kAhead];
     float x[kAhead][kPer];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
-      const int i = min(i0 + a * kPtWarps, last);
-      const size_t at = piece(i) * plan.rows + rr;
-      ml[a] = __ldcg(reinterpret_cast<const float2*>(plan.ml + at * 2));
+      const int i = i0 + a * kPtJoinWarps;
+      ml[a] = make_float2(kPtNothing, 0.f);
 #pragma unroll
-      for (int q = 0; q < kPer; ++q) x[a][q] = __ldcg(plan.o + at * D + lane + 32 * q);
+      for (int q = 0; q < kPer; ++q) x[a][q] = 0.f;
+      if (i <= last) {
+        const size_t at = piece(i) * plan.rows + rr;
+        ml[a] = __ldcg(reinterpret_cast<const float2*>(plan.ml + at * 2));
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) x[a][q] = __ldcg(plan.o + at * D + lane + 32 * q);
+      }
     }
     float mx = m;
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a)
-      if (i0 + a * kPtWarps <= last) mx = fmaxf(mx, ml[a].x);
-    const float f = m == mx ? 1.f : pt_exp2(m - mx);
+    for (int a = 0; a < kAhead; ++a) mx = fmaxf(mx, ml[a].x);
+    const float f = pt_exp2(m - mx);
     m = mx;
     l *= f;
 #pragma unroll
     for (int q = 0; q < kPer; ++q) acc[q] *= f;
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a)
-      if (i0 + a * kPtWarps <= last) {
-        const float w = ml[a].x == mx ? 1.f : pt_exp2(ml[a].x - mx);
-        l = fmaf(w, ml[a].y, l);
+    for (int a = 0; a < kAhead; ++a) {
+      const float w = pt_exp2(ml[a].x - mx);
+      l = fmaf(w, ml[a].y, l);
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) acc[q] = fmaf(w, x[a][q], acc[q]);
-      }
+      for (int q = 0; q < kPer; ++q) acc[q] = fmaf(w, x[a][q], acc[q]);
+    }
   }
 #pragma unroll
   for (int q = 0; q < kPer; ++q) so[warp][lane + 32 * q] = acc[q];
@@ -827,24 +923,20 @@ __global__ void __launch_bounds__(kPtThreads)
     sml[warp][1] = l;
   }
   __syncthreads();
-  float mx = -INFINITY, sum = 0.f, f[kPtWarps];
+  if (2 * tid >= D) return;
+  float mx = kPtNothing, sum = 0.f, a0 = 0.f, a1 = 0.f;
 #pragma unroll
-  for (int w = 0; w < kPtWarps; ++w) mx = fmaxf(mx, sml[w][0]);
+  for (int w = 0; w < kPtJoinWarps; ++w) mx = fmaxf(mx, sml[w][0]);
 #pragma unroll
-  for (int w = 0; w < kPtWarps; ++w) {
-    f[w] = sml[w][0] == mx ? 1.f : pt_exp2(sml[w][0] - mx);
-    sum = fmaf(f[w], sml[w][1], sum);
+  for (int w = 0; w < kPtJoinWarps; ++w) {
+    const float f = pt_exp2(sml[w][0] - mx);
+    const float2 x = *reinterpret_cast<const float2*>(&so[w][2 * tid]);
+    sum = fmaf(f, sml[w][1], sum);
+    a0 = fmaf(f, x.x, a0);
+    a1 = fmaf(f, x.y, a1);
   }
   const float inv = sum == 0.f ? 0.f : (p.v_scale ? p.v_scale[kvh] : 1.f) / sum;
-  for (int d = 2 * tid; d < D; d += 2 * kPtThreads) {
-    float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < kPtWarps; ++w) {
-      a0 = fmaf(f[w], so[w][d], a0);
-      a1 = fmaf(f[w], so[w][d + 1], a1);
-    }
-    *reinterpret_cast<uint32_t*>(p.out + row * D + d) = pt_pack<false>(a0 * inv, a1 * inv);
-  }
+  *reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(row) * D + 2 * tid) = pt_pack<false>(a0 * inv, a1 * inv);
   if (tid == 0 && p.lse) p.lse[row] = (mx + log2f(sum)) * 0.6931471805599453f;
 }
 
@@ -854,13 +946,13 @@ __global__ void __launch_bounds__(kPtThreads)
 namespace {
 
 struct PtChoice {
-  int nb, nchunk, groups, rows, tile, ctas_per_sm;
+  int nb, nchunk, groups, rows, tile_log, ctas_per_sm;
 };
 
 template <int D, int NB, bool F8>
 PtChoice pt_sizes() {
   using S = PtShape<D, NB, F8>;
-  return {NB, 1, 1, 8 * NB, kPtWarps * S::kKeys, S::kCtas};
+  return {NB, 1, 1, 8 * NB, S::kKeys == 32 ? 7 : 6, S::kCtas};
 }
 
 // As many 8-row blocks per warp as there are, up to what the registers hold; then one chunk of rows
@@ -946,6 +1038,7 @@ cudaError_t pt_launch(const PagedAttnParams& p, const PagedAttnPlan& plan, int n
   }
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(p.seq.B) * p.seq.T * p.Hq));
+  cfg.blockDim = dim3(32 * kPtJoinWarps);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, p, plan);
 }
@@ -969,7 +1062,8 @@ cudaError_t paged_attn_launch(const PagedAttnParams& p, bool f8, void* ws, int n
   if (dev < 0 || dev >= 64 || n_sm < 1) return cudaErrorInvalidDevice;
   const PtChoice c = pt_choose(p.seq.T, p.Hq, p.Hkv, p.D, f8);
   PagedAttnPlan plan;
-  plan.tile = c.tile;
+  plan.tile_log = c.tile_log;
+  plan.lead = kPtLead;
   plan.shift = -1;
   for (int i = 0; i < 31; ++i)
     if (p.seq.page == 1 << i) plan.shift = i;
