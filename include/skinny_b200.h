@@ -426,8 +426,8 @@ int skinny_paged_errors(void* dst, int clear, void* stream);
  * needs no initialisation. */
 size_t skinny_token_logprobs_workspace_bytes(int rows, int V, int top);
 
-/* Log probabilities under rows of logits x [rows, V] (type 0: bf16, 1: f32; row stride ld, rows need
- * only their element's alignment):
+/* Log probabilities under rows of logits x [rows, V] (type 0: bf16, 1: f32; V <= 2^27; row stride ld,
+ * rows need only their element's alignment):
  *   logprobs[r] = x[r, tokens[r]] - lse_r, lse_r = ln sum_v exp x[r, v]; -inf for a token outside
  *                 [0, V) (e.g. -1: none)
  *   entropy[r]  = -sum p ln p  (nats)

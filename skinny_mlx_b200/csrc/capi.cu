@@ -701,7 +701,7 @@ int skinny_paged_errors(void* dst, int clear, void* stream) {
 
 // ---- log probabilities ----
 size_t skinny_token_logprobs_workspace_bytes(int rows, int V, int top) {
-  if (rows < 1 || V < 1 || top < 0 || top > skinny::kLpMaxTop || top > V) return 0;
+  if (rows < 1 || V < 1 || V > skinny::kLpMaxVocab || top < 0 || top > skinny::kLpMaxTop || top > V) return 0;
   return skinny::logprob_ws_bytes(rows, V, top, skinny::device_sm_count(current_device()));
 }
 

@@ -9,16 +9,26 @@
 // -inf.
 //
 // One pass over the logits: every thread keeps a running maximum and the two sums relative to it in
-// f32 (renewed when a 16-byte piece exceeds it).  Bound by the bytes of the logits; next comes the
-// exponential unit (16 per clock and SM, where a bf16 stream at full bandwidth wants 12).
+// f32 (renewed when a 16-byte piece exceeds it).  With y = x log2(e) - M, M = fl(m log2(e)), e^(x - m) is 2^y
+// up to one common factor, the rounding of M, which a thread takes back at its end.  So a logit costs an fma
+// in f32, an exponential, an addition and an fma (pairs in one instruction each), half a maximum and half
+// a bound (pairs of bf16) and its unpacking.  Bound by the bytes of the logits; the exponential unit (16 per
+// clock and SM) would take 0.75 of that time.
 //
-// Alternatives.  A logit and its index form one 64-bit key whose order is the order wanted; keys are
-// all different.  The first pieces of four runs that a CTA's part of the row is read in (up to 8192 logits, in
-// registers) give a threshold that at least n keys reach: the n-th largest of the maxima of 64 groups.  After that, a
-// piece costs one comparison; what reaches the threshold, some n * (part / sample) logits, is put on a
-// list in shared memory, which is cut down by the same group maxima and ranked.  Rows whose order
-// defeats the threshold (rising logits) overflow the list: the part is then read again to find the
-// n-th key 12 bits at a time (a histogram per pass), which no input makes longer than 6 passes.
+// The bound: logits below -1e30 count as -1e30, so that 0 times y is 0 for a masked logit.  A part whose
+// maximum is beyond 1e6 in size (nothing but masks, most likely) is summed again with x - m: M is off by
+// up to 2^-24 of itself, and 2^y by as many powers of two.
+//
+// Alternatives.  A logit and its index form one 64-bit key whose order is the order wanted; keys are all
+// different.  In the pass a thread only keeps its largest logit and where it was (three instructions
+// per piece).  After it, the n-th largest of the maxima of 64 groups of threads is a threshold that at
+// least n keys reach and hardly more do; only (thread, run) pairs whose maximum reaches it, some n of 1024,
+// can hold such keys, and all threads together read those pairs' pieces again (2 % of the row at n = 20,
+// mostly from L2), put what reaches the threshold on a list and rank it.  (A list filled in the pass, behind a threshold from a
+// sample, cost 24 of 53 us at 509 rows and n = 20: half of a warp's steps had a logit for it.)
+// Rows that defeat the threshold (a thread whose logits are all large) overflow the list, and rows with
+// a NaN have no maxima to go by: the part is then read again to find the n-th key 12 bits at a time (a
+// histogram per pass), which no input makes longer than 6 passes.
 //
 // Few rows: a row is cut into parts, one CTA each, and a second launch joins their sums and lists.
 #include <algorithm>
@@ -37,7 +47,7 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpGroups = 64;      // groups whose maxima give a threshold (at least kLpMaxTop)
 constexpr int kLpList = 2048;      // keys a CTA's list holds
 constexpr int kLpRank = 128;       // keys that are ranked against each other
-constexpr int kLpSample = 4;       // 16-byte pieces per thread of the sample
+constexpr int kLpRuns = 4;         // 16-byte pieces per thread and step, from as many places of the part
 constexpr int kLpRadix = 12;       // bits per pass of the search for the n-th key
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLpLow = -3.402823466e38f;
@@ -71,25 +81,54 @@ __device__ __forceinline__ float lp_max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+__device__ __forceinline__ uint32_t lp_max_nan2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+constexpr float kLpMasked = -1e30f;               // the bound
+constexpr uint32_t kLpMasked2 = 0xF14AF14Au;      // a pair of bf16 below it, -1.0003e30
+constexpr float kLpFar = 1e6f;                    // maxima beyond it: M is too coarse
 
-// Running maximum (of numbers) and sums of e = e^(x - m) and e (x - m).
+// Running maximum (of numbers) and the sums of e = e^(x - m) and e (x - m).
 struct LpSums {
   float m = kLpLow, z = 0.f, s = 0.f;
-  // to maximum n >= m: z -> z f, s -> f (s + z (m - n)), f = e^(m - n)
-  __device__ __forceinline__ void renew(float n) {
-    const float d = m - n, f = lp_exp2(d * kLog2e);
+  // to a maximum n >= m: z -> z f, s -> f (s + z (m - n)), f = e^(m - n); unit: how d becomes a power of two
+  __device__ __forceinline__ void scale(float d, float unit) {
+    const float f = lp_exp2(d * unit);
     s = z == 0.f ? 0.f : f == 0.f && z == z && s == s ? 0.f : f * fmaf(z, d, s);
     z *= f;
+  }
+  __device__ __forceinline__ void renew(float n) {
+    scale(m - n, kLog2e);
     m = n;
   }
-  __device__ __forceinline__ void join(float om, float oz, float os) {
-    LpSums o;
-    o.m = om, o.z = oz, o.s = os;
-    const float n = fmaxf(m, om);
-    renew(n);
-    o.renew(n);
-    z += o.z;
-    s += o.s;
+  // a logit, whatever it is; d is bounded below so that 0 times an infinite d is 0 (NaN stays NaN)
+  __device__ __forceinline__ void add(float x) {
+    if (x > m) renew(x);
+    const float d = lp_max_nan(x - m, -1e4f), e = lp_exp2(d * kLog2e);
+    z += e;
+    s = fmaf(e, d, s);
+  }
+};
+
+// The same in the loop: M = fl(m log2(e)), sums of 2^y and 2^y y, y = x log2(e) - M, of bounded logits.
+struct LpFast {
+  float m = -2.f * kLpFar, M = -2.f * kLpFar * kLog2e;
+  LpSums a;
+  __device__ __forceinline__ void renew(float n) {
+    const float N = n * kLog2e;
+    a.scale(M - N, 1.f);
+    m = n;
+    M = N;
+  }
+  __device__ __forceinline__ LpSums sums() const {
+    const float r = fmaf(m, kLog2e, -M), f = lp_exp2(-r);  // 2^y = e^(x - m) 2^r
+    LpSums b;
+    b.m = m;
+    b.z = a.z * f;
+    b.s = f * fmaf(a.z, -r, a.s) * 0.6931471805599453f;
+    return b;
   }
 };
 
@@ -97,40 +136,47 @@ struct LpSums {
 template <bool F32>
 struct LpPiece {
   static constexpr int kN = F32 ? 4 : 8;
-  float x[kN];
-  __device__ __forceinline__ explicit LpPiece(const uint4& w) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (F32) {
-        x[i] = __uint_as_float(u[i]);
-      } else {
-        x[(F32 ? 0 : 2) * i] = __uint_as_float(u[i] << 16);
-        x[(F32 ? 0 : 2) * i + (F32 ? 0 : 1)] = __uint_as_float(u[i] & 0xFFFF0000u);
-      }
-    }
+  uint32_t u[4];
+  __device__ __forceinline__ explicit LpPiece(const uint4& w) : u{w.x, w.y, w.z, w.w} {}
+  __device__ __forceinline__ static float half(uint32_t w, int hi) {
+    return __uint_as_float(hi ? w & 0xFFFF0000u : w << 16);
+  }
+  __device__ __forceinline__ float at(int i) const { return F32 ? __uint_as_float(u[i & 3]) : half(u[i >> 1 & 3], i & 1); }
+  // The same for an index that the compiler does not know.
+  __device__ __forceinline__ float pick(int i) const {
+    const int k = F32 ? i : i >> 1;
+    const uint32_t w = k & 2 ? (k & 1 ? u[3] : u[2]) : (k & 1 ? u[1] : u[0]);
+    return F32 ? __uint_as_float(w) : half(w, i & 1);
   }
   // The largest, NaN above every number.
   __device__ __forceinline__ float top() const {
-    float t = x[0];
-#pragma unroll
-    for (int i = 1; i < kN; ++i) t = lp_max_nan(t, x[i]);
-    return t;
+    if (F32)
+      return lp_max_nan(lp_max_nan(__uint_as_float(u[0]), __uint_as_float(u[1])),
+                        lp_max_nan(__uint_as_float(u[2]), __uint_as_float(u[3])));
+    const uint32_t t = lp_max_nan2(lp_max_nan2(u[0], u[1]), lp_max_nan2(u[2], u[3]));
+    return lp_max_nan(half(t, 0), half(t, 1));
   }
-  __device__ __forceinline__ void add(LpSums& a, float top) const {
-    if (top > a.m) a.renew(top);
-    // d is bounded below so that 0 times an infinite d (a logit of -inf) is 0; NaN stays NaN
+  __device__ __forceinline__ LpPiece bounded() const {
+    LpPiece b = *this;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      b.u[i] = F32 ? __float_as_uint(lp_max_nan(__uint_as_float(u[i]), kLpMasked)) : lp_max_nan2(u[i], kLpMasked2);
+    return b;
+  }
+  // A bounded piece with largest logit `top` to the sums.
+  __device__ __forceinline__ void add(LpFast& f, float top) const {
+    if (top > f.m) f.renew(top);
+    LpSums& a = f.a;
     uint64_t z2 = f2_pack(0.f, 0.f), s2 = z2;
-    const uint64_t nm = f2_pack(-a.m, -a.m), one = f2_pack(1.f, 1.f), l2 = f2_pack(kLog2e, kLog2e);
+    const uint64_t nm = f2_pack(-f.M, -f.M), one = f2_pack(1.f, 1.f), l2 = f2_pack(kLog2e, kLog2e);
 #pragma unroll
     for (int i = 0; i < kN; i += 2) {
-      float d0, d1, a0, a1;
-      f2_unpack(f2_fma(f2_pack(x[i], x[i + 1]), one, nm), d0, d1);
-      const uint64_t d = f2_pack(lp_max_nan(d0, -1e4f), lp_max_nan(d1, -1e4f));
-      f2_unpack(f2_mul(d, l2), a0, a1);
-      const uint64_t e = f2_pack(lp_exp2(a0), lp_exp2(a1));
+      float y0, y1;
+      const uint64_t y = f2_fma(f2_pack(at(i), at(i + 1)), l2, nm);
+      f2_unpack(y, y0, y1);
+      const uint64_t e = f2_pack(lp_exp2(y0), lp_exp2(y1));
       z2 = f2_fma(e, one, z2);
-      s2 = f2_fma(e, d, s2);
+      s2 = f2_fma(e, y, s2);
     }
     float a0, a1;
     f2_unpack(z2, a0, a1);
@@ -142,7 +188,8 @@ struct LpPiece {
 
 struct LpPlan {
   int parts, part;            // CTAs per row, logits of one part
-  unsigned long long* keys;   // [rows, parts, top]
+  int cap;                    // keys of one part: its n largest among them, 0 where there are fewer
+  unsigned long long* keys;   // [rows, parts, cap]
   float* sums;                // [rows, parts, 4]: m, z, s
 };
 
@@ -150,6 +197,8 @@ struct LpSmem {
   unsigned long long list[2][kLpList];
   unsigned long long group[kLpGroups];
   int count[2];
+  int chosen[kLpRuns * kLpThreads];  // (run, thread) pairs whose pieces are read again
+  int n_chosen;
   int scan[kLpWarps];
   unsigned long long threshold;
 };
@@ -266,39 +315,65 @@ __device__ __noinline__ void lp_search(LpSmem& sm, const void* row, int c0, int 
 
 // What a row's sums and alternatives become.
 __device__ __forceinline__ float lp_logprob(float v, float m, float z, float lz) {
-  if (z != z) return v * 0.f + z;  // NaN
+  if (z != z) return z;
   return v == -INFINITY ? -INFINITY : v - m - lz;
 }
 
+// The given token's logit (asked for at a kernel's start: two dependent loads).
 template <bool F32>
-__device__ __forceinline__ void lp_finish(const LogprobParams& p, int row, const void* x, const LpSums& a) {
-  const float lz = logf(a.z);
+__device__ __forceinline__ float lp_token(const LogprobParams& p, int row, const void* x, bool& in) {
   const int t = p.tokens[row];
-  float v = -INFINITY;
-  const bool in = t >= 0 && t < p.V;
-  if (in) v = F32 ? static_cast<const float*>(x)[t] : __bfloat162float(static_cast<const __nv_bfloat16*>(x)[t]);
+  in = t >= 0 && t < p.V;
+  if (!in) return -INFINITY;
+  return F32 ? static_cast<const float*>(x)[t] : __bfloat162float(static_cast<const __nv_bfloat16*>(x)[t]);
+}
+
+__device__ __forceinline__ void lp_finish(const LogprobParams& p, int row, float v, bool in, const LpSums& a) {
+  const float lz = logf(a.z);
   p.logprob[row] = in ? lp_logprob(v, a.m, a.z, lz) : -INFINITY;
   p.entropy[row] = a.z == 0.f ? 0.f : lz - a.s / a.z;
 }
 
+// All threads' sums as one, in every thread.
 __device__ __forceinline__ void lp_block_sums(float (&red)[3][kLpWarps], LpSums& a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float m = a.m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
-    a.join(__shfl_xor_sync(0xFFFFFFFFu, a.m, o), __shfl_xor_sync(0xFFFFFFFFu, a.z, o), __shfl_xor_sync(0xFFFFFFFFu, a.s, o));
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  if (lane == 0) red[0][warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kLpWarps; ++w) m = fmaxf(m, red[0][w]);
+  a.renew(m);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, o);
+    a.s += __shfl_xor_sync(0xFFFFFFFFu, a.s, o);
+  }
   if (lane == 0) {
-    red[0][warp] = a.m;
     red[1][warp] = a.z;
     red[2][warp] = a.s;
   }
   __syncthreads();
-  a.m = red[0][0], a.z = red[1][0], a.s = red[2][0];
+  a.z = a.s = 0.f;
 #pragma unroll
-  for (int w = 1; w < kLpWarps; ++w) a.join(red[0][w], red[1][w], red[2][w]);
+  for (int w = 0; w < kLpWarps; ++w) {
+    a.z += red[1][w];
+    a.s += red[2][w];
+  }
+}
+
+// A part summed with x - m, logit by logit.
+template <bool F32>
+__device__ __noinline__ LpSums lp_careful(const void* row, int c0, int c1) {
+  LpSums a;
+  for (int i = c0 + threadIdx.x; i < c1; i += kLpThreads)
+    a.add(F32 ? static_cast<const float*>(row)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(row)[i]));
+  return a;
 }
 
 template <bool F32, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprob_part_kernel(const __grid_constant__ LogprobParams p,
+__global__ void __launch_bounds__(kLpThreads, 4) logprob_part_kernel(const __grid_constant__ LogprobParams p,
                                                                   const __grid_constant__ LpPlan plan) {
   constexpr int kN = LpPiece<F32>::kN, kEs = F32 ? 4 : 2;
   __shared__ float red[3][kLpWarps];
@@ -308,8 +383,12 @@ __global__ void __launch_bounds__(kLpThreads) logprob_part_kernel(const __grid_c
   const uint8_t* const x = static_cast<const uint8_t*>(p.x) + static_cast<long long>(row) * p.ld * kEs;
   const int c0 = blockIdx.x * plan.part, c1 = min(p.V, c0 + plan.part);
   pdl_launch_dependents();
-  if (TOP && tid == 0) sm.count[0] = 0;
+  if (TOP && tid == 0) sm.count[0] = sm.n_chosen = 0;
   pdl_wait_prior_grid();
+  const bool alone = plan.parts == 1;
+  bool in = false;
+  float tv = 0.f;
+  if (alone && tid == 0) tv = lp_token<F32>(p, row, x, in);
   // [a0, a1): whole 16-byte pieces; what lies before and after them is read one by one, at most 2 kN - 2
   const int mis = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) + static_cast<size_t>(c0) * kEs) % 16) % 16) / kEs;
   const int a0 = min(c1, c0 + mis), pieces = (c1 - a0) / kN, a1 = a0 + pieces * kN;
@@ -318,96 +397,120 @@ __global__ void __launch_bounds__(kLpThreads) logprob_part_kernel(const __grid_c
   const bool has_edge = edge < c1 && (edge < a0 || edge >= a1);
   float ev = -INFINITY;
   if (has_edge) ev = F32 ? reinterpret_cast<const float*>(x)[edge] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[edge]);
-  LpSums sums;
+  LpFast fast;
   const uint4 none = F32 ? make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u)
                          : make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);  // -inf
-  // the part as kLpSample runs, read side by side: the first pieces of each are the sample
-  const int runs = (pieces + kLpSample * kLpThreads - 1) / (kLpSample * kLpThreads) * kLpThreads;
-  uint4 w[kLpSample];
-  const auto load = [&](int base) {
+  // the part as kLpRuns runs, read side by side
+  const int runs = (pieces + kLpRuns * kLpThreads - 1) / (kLpRuns * kLpThreads) * kLpThreads;
+  uint4 w[kLpRuns];
+  const auto load = [&](uint4 (&v)[kLpRuns], int base) {
 #pragma unroll
-    for (int u = 0; u < kLpSample; ++u) {
+    for (int u = 0; u < kLpRuns; ++u) {
       const int i = u * runs + base + tid;
-      w[u] = i < pieces ? __ldcs(body + i) : none;
+      v[u] = i < pieces && base < runs ? __ldcs(body + i) : none;
     }
   };
-  load(0);
-  if (has_edge) {
-    if (ev > sums.m) sums.renew(ev);
-    const float d = lp_max_nan(ev - sums.m, -1e4f), e = lp_exp2(d * kLog2e);
-    sums.z += e;
-    sums.s = fmaf(e, d, sums.s);
-  }
-  unsigned long long threshold = 0;
-  float level = 0.f;  // the threshold's value: a piece below it has nothing for the list
-  bool any = true;    // the threshold is a NaN, or there is none
-  const auto offer = [&](const LpPiece<F32>& q, int i, int stop) {
+  load(w, 0);
+  float best = kLpMasked;  // this thread's largest logit above the bound, and its piece
+  int best_at = tid;
+  float run_best[kLpRuns];  // the same of its pieces of each run
 #pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      const unsigned long long key = lp_key(q.x[e], a0 + i * kN + e);
-      if (key >= threshold && i < stop) {
-        const int at = atomicAdd(&sm.count[0], 1);
-        if (at < kLpList) sm.list[0][at] = key;
-      }
-    }
-  };
-  if (TOP) {
-    unsigned long long best = has_edge ? lp_key(ev, edge) : 0;
-#pragma unroll
-    for (int u = 0; u < kLpSample; ++u) {
-      const int i = u * runs + tid;
-      if (i >= pieces) break;
-      const LpPiece<F32> q(w[u]);
-      const float t = q.top();
-      int at = kN;
-#pragma unroll
-      for (int e = kN - 1; e >= 0; --e)
-        if (q.x[e] == t || (t != t && q.x[e] != q.x[e])) at = e;
-      const unsigned long long key = lp_key(t, a0 + i * kN + at);
-      best = key > best ? key : best;
-    }
-    threshold = lp_threshold(sm, best, p.top);
-    level = lp_value(threshold);
-    any = threshold == 0 || level != level;
-    if (has_edge && lp_key(ev, edge) >= threshold) {
-      const int at = atomicAdd(&sm.count[0], 1);
-      if (at < kLpList) sm.list[0][at] = lp_key(ev, edge);
-    }
-  }
+  for (int u = 0; u < kLpRuns; ++u) run_best[u] = kLpMasked;
   for (int base = 0; base < runs; base += kLpThreads) {
-    if (base > 0) load(base);
+    uint4 next[kLpRuns];
+    load(next, base + kLpThreads);  // in flight while this step's pieces are added
 #pragma unroll
-    for (int u = 0; u < kLpSample; ++u) {
-      const LpPiece<F32> q(w[u]);
-      const float t = q.top();
-      if (TOP && (any || !(t < level))) offer(q, u * runs + base + tid, pieces);
-      q.add(sums, t);
+    for (int u = 0; u < kLpRuns; ++u) {
+      const LpPiece<F32> b = LpPiece<F32>(w[u]).bounded();
+      const float t = b.top();
+      if (TOP && t > best) {
+        best = t;
+        best_at = u * runs + base + tid;
+      }
+      if (TOP) run_best[u] = fmaxf(run_best[u], t);
+      b.add(fast, t);
     }
+#pragma unroll
+    for (int u = 0; u < kLpRuns; ++u) w[u] = next[u];
   }
-  const bool alone = plan.parts == 1;
+  LpSums sums = fast.sums();
+  if (has_edge) sums.add(lp_max_nan(ev, kLpMasked));
   lp_block_sums(red, sums);
+  if (!(sums.m > -kLpFar && sums.m < kLpFar)) {  // nothing but masks, or logits far from 0
+    sums = lp_careful<F32>(x, c0, c1);
+    __syncthreads();
+    lp_block_sums(red, sums);
+  }
   if (tid == 0) {
-    if (alone) lp_finish<F32>(p, row, x, sums);
+    if (alone) lp_finish(p, row, tv, in, sums);
     else *reinterpret_cast<float4*>(plan.sums + (static_cast<size_t>(row) * plan.parts + blockIdx.x) * 4) =
         make_float4(sums.m, sums.z, sums.s, 0.f);
   }
   if (TOP) {
+    // The threshold, from a key each thread's logits reach: its largest logit at the end of its piece (a
+    // thread of masked logits: -inf).
+    const bool some = best_at < pieces, above = best > kLpMasked;
+    unsigned long long low = some ? lp_key(above ? best : -INFINITY, a0 + best_at * kN + kN - 1) : 0;
+    const unsigned long long edge_key = has_edge ? lp_key(ev, edge) : 0;
+    low = edge_key > low ? edge_key : low;
+    const unsigned long long threshold = lp_threshold(sm, low, p.top);
+    const float level = threshold == 0 ? -INFINITY : lp_value(threshold);
+    // what can hold keys reaching it: a thread's pieces of a run; all where masked logits reach it
+#pragma unroll
+    for (int u = 0; u < kLpRuns; ++u)
+      if (u * runs + tid < pieces &&
+          (level <= kLpMasked || (run_best[u] > kLpMasked && lp_key(run_best[u], a0 + (u * runs + tid) * kN) >= threshold)))
+        sm.chosen[atomicAdd(&sm.n_chosen, 1)] = u * runs + tid;
+    if (edge_key != 0 && edge_key >= threshold) sm.list[0][atomicAdd(&sm.count[0], 1)] = edge_key;
+    __syncthreads();
+    const bool search = sums.z != sums.z;  // a NaN
+    const int steps = runs / kLpThreads, again = search ? 0 : sm.n_chosen * steps;
+    for (int q0 = 0; q0 < again; q0 += kLpRuns * kLpThreads) {
+      int at[kLpRuns];
+#pragma unroll
+      for (int u = 0; u < kLpRuns; ++u) {
+        const int q = q0 + u * kLpThreads + tid, who = q / steps, step = q - who * steps;
+        at[u] = q < again ? sm.chosen[who] + step * kLpThreads : pieces;
+        w[u] = at[u] < pieces ? __ldg(body + at[u]) : none;
+      }
+#pragma unroll
+      for (int u = 0; u < kLpRuns; ++u) {
+        const LpPiece<F32> q(w[u]);
+        if (at[u] >= pieces || q.top() < level) continue;
+        uint32_t hits = 0;
+#pragma unroll
+        for (int e = 0; e < kN; ++e) hits |= static_cast<uint32_t>(!(q.at(e) < level)) << e;
+        for (; hits; hits &= hits - 1) {
+          const int e = __ffs(hits) - 1;
+          const unsigned long long key = lp_key(q.pick(e), a0 + at[u] * kN + e);
+          if (key >= threshold) {
+            const int slot = atomicAdd(&sm.count[0], 1);
+            if (slot < kLpList) sm.list[0][slot] = key;
+          }
+        }
+      }
+    }
     __syncthreads();
     int cnt = sm.count[0];
-    if (cnt > kLpList) {
+    if (search || cnt > kLpList) {
       lp_search<F32>(sm, x, c0, c1, p.top);
       cnt = sm.count[0];
     }
-    const float lz = logf(sums.z);
-    unsigned long long* const keys = plan.keys + (static_cast<size_t>(row) * plan.parts + blockIdx.x) * p.top;
-    if (!alone && tid < p.top && tid >= cnt) keys[tid] = 0;  // a part of fewer logits than alternatives
-    lp_rank(sm, cnt, p.top, [&](int rank, unsigned long long key) {
-      if (alone) {
-        p.top_id[static_cast<size_t>(row) * p.top + rank] = lp_index(key);
-        p.top_lp[static_cast<size_t>(row) * p.top + rank] = lp_logprob(lp_value(key), sums.m, sums.z, lz);
+    if (!alone) {
+      // the keys as they are where they are few; the join ranks them
+      unsigned long long* const keys = plan.keys + (static_cast<size_t>(row) * plan.parts + blockIdx.x) * plan.cap;
+      if (cnt <= plan.cap) {
+        if (tid < plan.cap) keys[tid] = tid < cnt ? sm.list[0][tid] : 0;
       } else {
-        keys[rank] = key;
+        if (tid >= p.top && tid < plan.cap) keys[tid] = 0;
+        lp_rank(sm, cnt, p.top, [&](int rank, unsigned long long key) { keys[rank] = key; });
       }
+      return;
+    }
+    const float lz = logf(sums.z);
+    lp_rank(sm, cnt, p.top, [&](int rank, unsigned long long key) {
+      p.top_id[static_cast<size_t>(row) * p.top + rank] = lp_index(key);
+      p.top_lp[static_cast<size_t>(row) * p.top + rank] = lp_logprob(lp_value(key), sums.m, sums.z, lz);
     });
   }
 }
@@ -421,45 +524,59 @@ __global__ void __launch_bounds__(kLpThreads) logprob_join_kernel(const __grid_c
   LpSmem& sm = reinterpret_cast<LpSmem&>(smem);  // (used where TOP)
   const int tid = threadIdx.x, row = blockIdx.x;
   pdl_launch_dependents();
+  if (TOP && tid == 0) sm.count[0] = 0;
+  if (TOP) __syncthreads();
   pdl_wait_prior_grid();
-  const int n = TOP ? plan.parts * p.top : 0;
-  if (TOP)
-    for (int i = tid; i < n; i += kLpThreads) sm.list[0][i] = __ldcg(plan.keys + static_cast<size_t>(row) * n + i);
+  bool in = false;
+  float tv = 0.f;
+  if (tid == 0)
+    tv = lp_token<F32>(p, row, static_cast<const uint8_t*>(p.x) + static_cast<long long>(row) * p.ld * (F32 ? 4 : 2), in);
   LpSums sums;
   if (tid < plan.parts) {
     const float4 v = __ldcg(reinterpret_cast<const float4*>(plan.sums) + static_cast<size_t>(row) * plan.parts + tid);
     sums.m = v.x, sums.z = v.y, sums.s = v.z;
   }
+  if (TOP) {
+    const int n = plan.parts * plan.cap;
+    const unsigned long long* const from = plan.keys + static_cast<size_t>(row) * n;
+    for (int i = tid; i < n; i += kLpThreads) {
+      const unsigned long long key = __ldcg(from + i);
+      if (key != 0) sm.list[0][atomicAdd(&sm.count[0], 1)] = key;
+    }
+  }
   lp_block_sums(red, sums);  // (a barrier: the list is there)
-  if (tid == 0)
-    lp_finish<F32>(p, row, static_cast<const uint8_t*>(p.x) + static_cast<long long>(row) * p.ld * (F32 ? 4 : 2), sums);
+  if (tid == 0) lp_finish(p, row, tv, in, sums);
   if (TOP) {
     const float lz = logf(sums.z);
-    lp_rank(sm, n, p.top, [&](int rank, unsigned long long key) {
+    lp_rank(sm, sm.count[0], p.top, [&](int rank, unsigned long long key) {
       p.top_id[static_cast<size_t>(row) * p.top + rank] = lp_index(key);
       p.top_lp[static_cast<size_t>(row) * p.top + rank] = lp_logprob(lp_value(key), sums.m, sums.z, lz);
     });
   }
 }
 
-// Parts per row: as many as give every SM some CTAs, of at least 4096 logits, and no more than the join's
-// list holds (and its threads read).
+// Parts per row.  From three rows per SM on a row is one CTA (509 rows with 20 alternatives: 42 us, in two
+// parts 45, in five 49: what a part and the join cost besides the logits); fewer rows are cut so that
+// every SM has four CTAs (300 f32 rows: one part 54 us, two 48), of at least 4096 logits, and no more than the
+// join's list holds and its threads read.
 static void lp_parts(int rows, int V, int top, int n_sm, LpPlan& plan) {
-  const int most = std::min({(V + 4095) / 4096, kLpThreads, top > 0 ? kLpList / top : kLpThreads});
-  const int want = (4 * std::max(n_sm, 1) + rows - 1) / rows;
+  plan.cap = top > 0 ? top + 32 : 0;
+  const int sms = std::max(n_sm, 1);
+  const int most = std::min({V / 4096 + (V % 4096 > 0), kLpThreads, top > 0 ? kLpList / plan.cap : kLpThreads});
+  const int want = rows >= 3 * sms ? 1 : (4 * sms + rows - 1) / rows;
   plan.parts = std::max(1, std::min(most, want));
-  plan.part = ((V + plan.parts - 1) / plan.parts + 63) / 64 * 64;
-  plan.parts = (V + plan.part - 1) / plan.part;
+  plan.part = ((V - 1) / plan.parts / 64 + 1) * 64;
+  plan.parts = (V - 1) / plan.part + 1;
 }
 
-static size_t lp_keys_bytes(int rows, int parts, int top) {
-  return (static_cast<size_t>(rows) * parts * top * 8 + 15) / 16 * 16;
+static size_t lp_keys_bytes(int rows, const LpPlan& plan) {
+  return (static_cast<size_t>(rows) * plan.parts * plan.cap * 8 + 15) / 16 * 16;
 }
 
 size_t logprob_ws_bytes(int rows, int V, int top, int n_sm) {
   LpPlan plan;
   lp_parts(rows, V, top, n_sm, plan);
-  return lp_keys_bytes(rows, plan.parts, top) + static_cast<size_t>(rows) * plan.parts * 16;
+  return plan.parts == 1 ? 16 : lp_keys_bytes(rows, plan) + static_cast<size_t>(rows) * plan.parts * 16;
 }
 
 template <bool F32, bool TOP>
@@ -483,7 +600,7 @@ static cudaError_t lp_launch(const LogprobParams& p, const LpPlan& plan, cudaStr
     q.entropy += r0;
     q.top_lp += static_cast<size_t>(r0) * p.top;
     q.top_id += static_cast<size_t>(r0) * p.top;
-    pl.keys += static_cast<size_t>(r0) * plan.parts * p.top;
+    pl.keys += static_cast<size_t>(r0) * plan.parts * plan.cap;
     pl.sums += static_cast<size_t>(r0) * plan.parts * 4;
     cfg.gridDim = dim3(plan.parts, q.rows);
     cudaError_t e = cudaLaunchKernelEx(&cfg, logprob_part_kernel<F32, TOP>, q, pl);
@@ -500,7 +617,7 @@ cudaError_t logprob_launch(const LogprobParams& p, bool f32, void* ws, int n_sm,
   LpPlan plan;
   lp_parts(p.rows, p.V, p.top, n_sm, plan);
   plan.keys = static_cast<unsigned long long*>(ws);
-  plan.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + lp_keys_bytes(p.rows, plan.parts, p.top));
+  plan.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + lp_keys_bytes(p.rows, plan));
   if (p.top > 0) return f32 ? lp_launch<true, true>(p, plan, stream) : lp_launch<false, true>(p, plan, stream);
   return f32 ? lp_launch<true, false>(p, plan, stream) : lp_launch<false, false>(p, plan, stream);
 }

@@ -5,7 +5,8 @@
 
 namespace skinny {
 
-constexpr int kLpMaxTop = 32;  // alternatives per row
+constexpr int kLpMaxTop = 32;           // alternatives per row
+constexpr int kLpMaxVocab = 1 << 27;    // logits per row
 
 struct LogprobParams {
   const void* x;  // [rows, V], row stride ld

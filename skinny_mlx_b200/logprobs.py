@@ -14,6 +14,7 @@ import torch
 from . import _lib
 
 MAX_TOP = 32
+MAX_VOCAB = 2**27
 _TYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
@@ -41,8 +42,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0) -
     if kind is None or logits.dim() != 2:
         raise ValueError("logits must be a bf16 or f32 [rows, V] tensor")
     rows, v = logits.shape
-    if v < 1 or v > 2**31 - 1 or (v > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < v):
-        raise ValueError("logits must have columns, unit column stride and rows that do not overlap")
+    if not 1 <= v <= MAX_VOCAB or (v > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < v):
+        raise ValueError(f"logits must have 1 to {MAX_VOCAB} columns, unit column stride and rows that do not overlap")
     if tokens.shape != (rows,) or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
         raise ValueError(f"tokens must be int32 or int64 [{rows}] on the logits' device")
     if not 0 <= top_n <= min(MAX_TOP, v):
@@ -51,20 +52,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0) -
     if tokens.dtype == torch.int64:  # ids beyond 32 bits are outside every vocabulary
         tokens = tokens.clamp(-1, 2**31 - 1).to(torch.int32)
     tokens = tokens.contiguous()
-    lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
+    lp = torch.empty(rows, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(lp)
     top = torch.empty(rows, top_n, dtype=torch.float32, device=dev)
     ids = torch.empty(rows, top_n, dtype=torch.int32, device=dev)
     if rows:
-        with torch.cuda.device(dev):
-            key = (dev.index, rows, v, top_n)
-            n = _ws_bytes.get(key)
-            if n is None:
+        key = (dev.index, rows, v, top_n)
+        n = _ws_bytes.get(key)
+        if n is None:
+            with torch.cuda.device(dev):
                 n = _ws_bytes[key] = int(_lib.lib().skinny_token_logprobs_workspace_bytes(rows, v, top_n))
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)  # scratch of this call alone
-            _lib.call("skinny_token_logprobs", logits.data_ptr(), logits.stride(0), kind, rows, v, tokens.data_ptr(), top_n,
-                      lp.data_ptr(), ent.data_ptr(), top.data_ptr(), ids.data_ptr(), ws.data_ptr(), n,
-                      torch.cuda.current_stream(dev).cuda_stream)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)  # scratch of this call alone
+        _lib.launch("skinny_token_logprobs", dev.index, logits.data_ptr(), logits.stride(0), kind, rows, v,
+                    tokens.data_ptr(), top_n, lp.data_ptr(), ent.data_ptr(), top.data_ptr(), ids.data_ptr(), ws.data_ptr(), n)
     return TokenLogprobs(lp, ent, top, ids)
 
 
-__all__ = ["token_logprobs", "TokenLogprobs", "MAX_TOP"]
+__all__ = ["token_logprobs", "TokenLogprobs", "MAX_TOP", "MAX_VOCAB"]

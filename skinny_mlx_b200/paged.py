@@ -37,14 +37,15 @@ _Strides = ctypes.c_longlong * 3
 def _rows(x: torch.Tensor, name: str, b: int, t: int, d: int, dev: torch.device) -> tuple[torch.Tensor, ctypes.Array]:
     """A bf16 [B, T, heads, D] input whose dims are dense and whose rows are 16-byte aligned (copied if
     they are not), and its strides."""
-    if x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[0] != b or x.shape[1] != t or x.shape[3] != d:
-        raise ValueError(f"{name} must be bf16 [{b}, {t}, heads, {d}], got {x.dtype} {tuple(x.shape)}")
+    shape = x.shape
+    if x.dtype != torch.bfloat16 or len(shape) != 4 or shape[0] != b or shape[1] != t or shape[3] != d:
+        raise ValueError(f"{name} must be bf16 [{b}, {t}, heads, {d}], got {x.dtype} {tuple(shape)}")
     if x.device != dev:
         raise ValueError(f"{name} is on {x.device}, the pages on {dev}")
     sb, st, sh, sd = x.stride()
     # the stride of an axis of one element says nothing
-    sb, st, sh = (0 if n == 1 else s for n, s in zip(x.shape, (sb, st, sh)))
-    if (d > 1 and sd != 1) or sb % 8 or st % 8 or sh % 8 or x.data_ptr() % 16:
+    sb, st, sh = 0 if b == 1 else sb, 0 if t == 1 else st, 0 if shape[2] == 1 else sh
+    if sd != 1 or (sb | st | sh) & 7 or x.data_ptr() & 15:
         x = x.clone(memory_format=torch.contiguous_format)
         sb, st, sh, _ = x.stride()
     return x, _Strides(sb, st, sh)
@@ -141,14 +142,12 @@ def append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages: to
     _seqs(block_table, lengths, counts, b, t, page, dev)
     if b == 0 or t == 0:
         return out
-    with torch.cuda.device(dev):
-        _lib.call("skinny_paged_append", q.data_ptr() if hq else None, qs, k.data_ptr(), ks, v.data_ptr(), vs,
-                  out.data_ptr() if hq else None, k_pages.data_ptr(), v_pages.data_ptr(), _page_stride(k_pages),
-                  _page_stride(v_pages), kv, None if k_scale is None else k_scale.data_ptr(),
-                  None if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                  block_table.shape[1], n_pages, page, lengths.data_ptr(), None if counts is None else counts.data_ptr(),
-                  inv_freq.data_ptr() if rot else None, rot, b, t, hq, hkv, d,
-                  torch.cuda.current_stream(dev).cuda_stream)
+    _lib.launch("skinny_paged_append", dev.index, q.data_ptr() if hq else None, qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                out.data_ptr() if hq else None, k_pages.data_ptr(), v_pages.data_ptr(), _page_stride(k_pages),
+                _page_stride(v_pages), kv, None if k_scale is None else k_scale.data_ptr(),
+                None if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                block_table.shape[1], n_pages, page, lengths.data_ptr(), None if counts is None else counts.data_ptr(),
+                inv_freq.data_ptr() if rot else None, rot, b, t, hq, hkv, d)
     return out
 
 
@@ -187,20 +186,19 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
     out = torch.empty(b, t, hq, d, dtype=torch.bfloat16, device=dev)
     lse = torch.empty(b, t, hq, dtype=torch.float32, device=dev) if return_lse else None
     if b and t:
-        with torch.cuda.device(dev):
-            key = (dev.index, b, t, hq, hkv, d)
-            n = _ws_bytes.get(key)
-            if n is None:
+        key = (dev.index, b, t, hq, hkv, d)
+        n = _ws_bytes.get(key)
+        if n is None:
+            with torch.cuda.device(dev):
                 n = _ws_bytes[key] = int(_lib.lib().skinny_paged_attn_workspace_bytes(b, t, hq, hkv, d))
-            # scratch of this call alone: calls on other streams and captured graphs have their own
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            _lib.call("skinny_paged_attn", q.data_ptr(), qs, k_pages.data_ptr(), v_pages.data_ptr(), _page_stride(k_pages),
-                      _page_stride(v_pages), kv, None if k_scale is None else k_scale.data_ptr(),
-                      None if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                      block_table.shape[1], n_pages, page, lengths.data_ptr(),
-                      None if counts is None else counts.data_ptr(), scale, window or 0, out.data_ptr(),
-                      None if lse is None else lse.data_ptr(), b, t, hq, hkv, d, ws.data_ptr(), n,
-                      torch.cuda.current_stream(dev).cuda_stream)
+        # scratch of this call alone: calls on other streams and captured graphs have their own
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        _lib.launch("skinny_paged_attn", dev.index, q.data_ptr(), qs, k_pages.data_ptr(), v_pages.data_ptr(),
+                    _page_stride(k_pages), _page_stride(v_pages), kv, None if k_scale is None else k_scale.data_ptr(),
+                    None if v_scale is None else v_scale.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                    block_table.shape[1], n_pages, page, lengths.data_ptr(),
+                    None if counts is None else counts.data_ptr(), scale, window or 0, out.data_ptr(),
+                    None if lse is None else lse.data_ptr(), b, t, hq, hkv, d, ws.data_ptr(), n)
     return (out, lse) if return_lse else out
 
 

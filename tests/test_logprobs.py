@@ -34,7 +34,7 @@ def test_refusals():
         return L.skinny_token_logprobs(logits, ld, kind, rows, v, tokens, top, lp, ent, tl, ti, ws, n, None)
 
     for kw, status in ((dict(logits=None), -1), (dict(tokens=None), -1), (dict(lp=None), -1), (dict(ent=None), -1),
-                       (dict(kind=2), -1), (dict(tl=None), -1), (dict(ti=None), -1), (dict(rows=0), -2), (dict(v=0), -2),
+                       (dict(kind=2), -1), (dict(tl=None), -1), (dict(ti=None), -1), (dict(rows=0), -2), (dict(v=0), -2), (dict(v=2**27 + 1, ld=2**28), -2),
                        (dict(top=33), -2), (dict(top=-1), -2), (dict(v=3, top=4), -2), (dict(ld=63), -2),
                        (dict(logits=f + 1), -4), (dict(logits=f + 2, kind=1), -4), (dict(tokens=f + 2), -4),
                        (dict(ws=None), -5), (dict(n=0), -5), (dict(ws=f + 8), -5)):
