@@ -25,7 +25,7 @@ import torch.nn.functional as F
 from torch.nn.attention import sdpa_kernel
 
 from .configs import DenseConfig
-from .model import _SDPA_BACKENDS, AttnCache, QuantizedLinear, RMSNorm, _rope
+from .model import _SDPA_BACKENDS, AttnCache, PagedAttnCache, QuantizedLinear, RMSNorm, _rope
 from .qmm import dequantize, quantize
 
 
@@ -89,24 +89,32 @@ class DenseLayer(nn.Module):
         q = qkv[:, :nq * D].reshape(T, nq, D)
         k = qkv[:, nq * D:(nq + nkv) * D].reshape(T, nkv, D)
         v = qkv[:, (nq + nkv) * D:].reshape(T, nkv, D)
-        pos = torch.arange(cache.length, cache.length + T, device=x.device)
-        q = _rope(self.q_norm(q).float(), pos, D, cfg.rope_theta).to(torch.bfloat16)
-        k = _rope(self.k_norm(k).float(), pos, D, cfg.rope_theta).to(torch.bfloat16)
-        L0 = cache.length
-        cache.k[L0:L0 + T] = k
-        cache.v[L0:L0 + T] = v
-        cache.length = L0 + T
-        causal = pos[:, None] >= torch.arange(L0 + T, device=x.device)[None, :]
-        with sdpa_kernel(_SDPA_BACKENDS):
-            o = F.scaled_dot_product_attention(q.transpose(0, 1)[None], cache.k[:L0 + T].transpose(0, 1)[None],
-                                               cache.v[:L0 + T].transpose(0, 1)[None], attn_mask=causal,
-                                               enable_gqa=True)[0].transpose(0, 1).reshape(T, nq * D)
+        if isinstance(cache, PagedAttnCache):
+            o = cache.attend(self.q_norm(q), self.k_norm(k), v, D, cfg.rope_theta).reshape(T, nq * D)
+        else:
+            o = self._attend(q, k, v, cache)
         o = ex.gather(o.to(torch.bfloat16))
         h = (x.float() + ex.gather(self.o_proj(o)).float()).to(torch.bfloat16)
         gu = self.gate_up_proj(self.post_attention_layernorm(h))
         half = gu.shape[1] // 2
         a = ex.gather((F.silu(gu[:, :half].float()) * gu[:, half:].float()).to(torch.bfloat16))
         return (h.float() + ex.gather(self.down_proj(a)).float()).to(torch.bfloat16)
+
+    def _attend(self, q, k, v, cache: AttnCache) -> torch.Tensor:
+        cfg, D, nq = self.cfg, self.cfg.head_dim, self.nq
+        T = q.shape[0]
+        pos = torch.arange(cache.length, cache.length + T, device=q.device)
+        q = _rope(self.q_norm(q).float(), pos, D, cfg.rope_theta).to(torch.bfloat16)
+        k = _rope(self.k_norm(k).float(), pos, D, cfg.rope_theta).to(torch.bfloat16)
+        L0 = cache.length
+        cache.k[L0:L0 + T] = k
+        cache.v[L0:L0 + T] = v
+        cache.length = L0 + T
+        causal = pos[:, None] >= torch.arange(L0 + T, device=q.device)[None, :]
+        with sdpa_kernel(_SDPA_BACKENDS):
+            return F.scaled_dot_product_attention(q.transpose(0, 1)[None], cache.k[:L0 + T].transpose(0, 1)[None],
+                                                  cache.v[:L0 + T].transpose(0, 1)[None], attn_mask=causal,
+                                                  enable_gqa=True)[0].transpose(0, 1).reshape(T, nq * D)
 
 
 class DenseModel(nn.Module):
@@ -131,8 +139,17 @@ class DenseModel(nn.Module):
         self.norm = RMSNorm(cfg.hidden, cfg.rms_eps)
         self.to(dev)
 
-    def make_cache(self, max_len: int = 4096) -> list[AttnCache]:
+    def make_cache(self, max_len: int = 4096, pool=None) -> list[AttnCache]:
+        """pool: a paged.PagePool of cfg.layers layers and this rank's kv heads, instead of contiguous buffers
+        (the caches' shared page table, `caches[0].table`, is released by the caller)."""
         c = self.cfg
+        if pool is not None:
+            from .paged import PageTable
+
+            if pool.k.shape[0] != c.layers or tuple(pool.k.shape[2::2]) != (c.n_kv_heads // self.world, c.head_dim):
+                raise ValueError("the pool has other layers or heads than the model")
+            table = PageTable(pool, max_len)
+            return [PagedAttnCache(pool, table, i) for i in range(c.layers)]
         shard = type("C", (), {"n_kv_heads": c.n_kv_heads // self.world, "head_dim": c.head_dim})
         return [AttnCache(shard, max_len, self.device) for _ in range(c.layers)]
 

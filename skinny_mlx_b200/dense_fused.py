@@ -38,6 +38,7 @@ import torch.distributed as dist
 
 from . import _lib
 from .dense import DenseModel
+from .model import PagedAttnCache
 from .qmm import get_workspace
 
 _KINDS = 4  # attention digits, o_proj shard, SwiGLU digits, down shard
@@ -249,6 +250,8 @@ class DenseFusedStep:
         """Logits [G, M, V/G] bf16 (rank-major shards of the vocabulary; a reused buffer)."""
         cfg, m, G = self.cfg, ids.shape[0], self.G
         assert 1 <= m <= 16
+        if any(isinstance(c, PagedAttnCache) for c in caches):
+            raise ValueError("the fused step reads contiguous caches: run the model on paged ones")
         b = self._buffers(m)
         dev = self.model.device
         stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)

@@ -184,6 +184,8 @@ class FusedStep(FusedOps):
         tokens (host list or device int32 tensor) for a draft-tree verify, which needs recording
         GDN caches (HybridRollback.record) and is followed by HybridRollback.rollback_tree."""
         cfg, m = self.cfg, ids.shape[0]
+        if getattr(cache, "table", None) is not None:
+            raise ValueError("the fused step reads contiguous caches: run the model on a paged one")
         if m > 16:  # prefill: the module-by-module forward (qmm in 16-token chunks)
             if tree is not None:
                 raise ValueError("a tree verify takes at most 16 tokens")
@@ -306,7 +308,7 @@ class GraphedStep:
     def __call__(self, ids: torch.Tensor, cache, tree=None):
         """tree: parents of the tokens (host list) for a draft-tree verify, else None."""
         m = ids.shape[0]
-        if m > 16:
+        if m > 16 or getattr(cache, "table", None) is not None:
             return self.fused(ids, cache, tree=tree)
         gdn = [c for c in cache.layers if isinstance(c, GDNCache)]
         key = (id(cache), m, tuple(c.recording for c in gdn), tree is not None)

@@ -177,6 +177,63 @@ class AttnCache:
         return n
 
 
+class PagedAttnCache(AttnCache):
+    """KV cache of one attention layer in pages of a pool (skinny_mlx_b200.paged) that several
+    sequences share; `table` is the sequence's page table, one for all its layers.  A length and a trim like
+    AttnCache's; there are no contiguous k and v, so the fused step and token trees do not take it."""
+
+    def __init__(self, pool, table, layer: int):
+        self.pool, self.table, self.layer, self.length = pool, table, layer, 0
+        self._len = torch.zeros(1, dtype=torch.int32, device=pool.k.device)
+
+    def gather(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The cached keys and values in order, [length, n_kv_heads, head_dim] bf16."""
+        out = []
+        n = -(-self.length // self.pool.page)
+        rows = self.table.device[0, :n].long()
+        for pages, scale in ((self.pool.k, self.pool.k_scale), (self.pool.v, self.pool.v_scale)):
+            x, s = pages[self.layer], scale[self.layer]
+            if s is not None:
+                x = (x.view(torch.uint8)[rows].view(x.dtype).float() * s[:, None, None]).to(torch.bfloat16)
+            else:
+                x = x[rows]
+            out.append(x.transpose(1, 2).reshape(-1, x.shape[1], x.shape[3])[:self.length])
+        return out[0], out[1]
+
+    def attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rot: int, theta: float) -> torch.Tensor:
+        """Append T new tokens (q, k normalised bf16 [T, heads, D], v bf16) and attend causally: o bf16
+        [T, n_heads, D].  Up to 16 tokens run on the paged kernels; a prompt is appended by the kernel and
+        attends over the gathered pages."""
+        from . import paged
+
+        T, L0 = q.shape[0], self.length
+        self.table.reserve(L0 + T)
+        self.length = L0 + T
+        kp, vp = self.pool.k[self.layer], self.pool.v[self.layer]
+        ks, vs = self.pool.k_scale[self.layer], self.pool.v_scale[self.layer]
+        if q.is_cuda:
+            self._len.fill_(L0)
+            inv = theta ** (-torch.arange(0, rot // 2, device=q.device, dtype=torch.float32) / (rot // 2)) if rot else None
+            q = paged.append(q[None], k[None], v[None], kp, vp, self.table.device, self._len, inv, k_scale=ks, v_scale=vs)
+            if T <= paged.MAX_TOKENS:
+                return paged.attention(q, kp, vp, self.table.device, self._len, k_scale=ks, v_scale=vs)[0]
+            q = q[0]
+        else:  # CPU runs (tests)
+            pos = torch.arange(L0, L0 + T)
+            q, k = (_rope(x.float(), pos, rot, theta).to(torch.bfloat16) for x in (q, k))
+            rows, slot = self.table.device[0].long()[pos // self.pool.page], pos % self.pool.page
+            for pages, x, s in ((kp, k, ks), (vp, v, vs)):
+                if s is not None:
+                    x = (x.float() / s[:, None]).clamp(-448, 448).to(pages.dtype).view(torch.uint8)
+                    pages = pages.view(torch.uint8)
+                pages[rows, :, slot] = x
+        kk, vv = self.gather()
+        causal = torch.arange(L0, L0 + T, device=q.device)[:, None] >= torch.arange(L0 + T, device=q.device)[None]
+        with sdpa_kernel(_SDPA_BACKENDS):
+            return F.scaled_dot_product_attention(q.transpose(0, 1)[None], kk.transpose(0, 1)[None], vv.transpose(0, 1)[None],
+                                                  attn_mask=causal, enable_gqa=True)[0].transpose(0, 1)
+
+
 class GDNCache:
     """Conv window, recurrent state and (while a verify is recorded) checkpoints of one GDN layer."""
 
@@ -194,10 +251,26 @@ class GDNCache:
 
 
 class Cache:
-    def __init__(self, model: "HybridModel", max_len: int = 4096, max_verify: int = 17):
+    """pool (a paged.PagePool for the model's attention layers): keys and values go to its pages instead of
+    contiguous buffers; release() gives them back."""
+
+    def __init__(self, model: "HybridModel", max_len: int = 4096, max_verify: int = 17, pool=None):
         cfg, dev = model.cfg, model.device
-        self.layers = [AttnCache(cfg, max_len, dev) if cfg.is_attention(i) else GDNCache(cfg, max_verify, dev)
-                       for i in range(cfg.layers)]
+        self.table = None
+        if pool is not None:
+            from .paged import PageTable
+
+            if pool.k.shape[0] != sum(cfg.is_attention(i) for i in range(cfg.layers)) or pool.k.device != torch.empty(
+                    0, device=dev).device or tuple(pool.k.shape[2::2]) != (cfg.n_kv_heads, cfg.head_dim):
+                raise ValueError("the pool has other layers, heads or another device than the model")
+            self.table = PageTable(pool, max_len)
+        attn = iter(range(cfg.layers))
+        self.layers = [(AttnCache(cfg, max_len, dev) if pool is None else PagedAttnCache(pool, self.table, next(attn)))
+                       if cfg.is_attention(i) else GDNCache(cfg, max_verify, dev) for i in range(cfg.layers)]
+
+    def release(self) -> None:
+        """Empty a paged cache and give its pages back to the pool."""
+        self.reset()
 
     @property
     def offset(self) -> int:
@@ -208,6 +281,8 @@ class Cache:
 
     def reset(self) -> None:
         """Empty the cache in place (same buffers: captured graphs that use it stay valid)."""
+        if self.table is not None:
+            self.table.release()
         for c in self.layers:
             if isinstance(c, AttnCache):
                 c.length = 0
@@ -278,6 +353,12 @@ class Attention(nn.Module):
         q, gate = qg[..., :D], qg[..., D:]
         k = k.reshape(T, nkv, D)
         v = v.reshape(T, nkv, D)
+        if isinstance(cache, PagedAttnCache):
+            if tree is not None:
+                raise ValueError("a tree verify needs a contiguous cache")
+            o = cache.attend(self.q_norm(q), self.k_norm(k), v, cfg.rotary_dim, cfg.rope_theta)
+            o = o.float() * torch.sigmoid(gate.float())
+            return o.reshape(T, nh * D).to(torch.bfloat16)
         L0 = cache.length
         if tree is None:
             pos = torch.arange(L0, L0 + T, device=qg.device)
@@ -452,8 +533,16 @@ class HybridModel(nn.Module):
         self.norm = RMSNorm(cfg.hidden, cfg.rms_eps)
         self.to(self.device)
 
-    def make_cache(self, max_len: int = 4096, max_verify: int = 17) -> Cache:
-        return Cache(self, max_len, max_verify)
+    def make_cache(self, max_len: int = 4096, max_verify: int = 17, pool=None) -> Cache:
+        return Cache(self, max_len, max_verify, pool)
+
+    def make_pool(self, n_pages: int, page: int = 64, **kw):
+        """A page pool for this model's attention layers (paged.PagePool), to be shared by several caches."""
+        from .paged import PagePool
+
+        cfg = self.cfg
+        return PagePool(sum(cfg.is_attention(i) for i in range(cfg.layers)), n_pages, cfg.n_kv_heads, cfg.head_dim, page,
+                        device=self.device, **kw)
 
     @torch.no_grad()
     def forward(self, ids: torch.Tensor, cache: Cache, tree=None):
@@ -467,4 +556,4 @@ class HybridModel(nn.Module):
 
 __all__ = ["ModelConfig", "config3", "SMALL", "HybridModel", "QuantizedLinear", "QuantizedEmbedding", "tree_paths",
            "tree_rows",
-           "Cache", "AttnCache", "GDNCache", "RMSNorm", "DecoderLayer", "Attention", "GatedDeltaNet", "MLP"]
+           "Cache", "AttnCache", "PagedAttnCache", "GDNCache", "RMSNorm", "DecoderLayer", "Attention", "GatedDeltaNet", "MLP"]

@@ -202,6 +202,74 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
     return (out, lse) if return_lse else out
 
 
+class PagePool:
+    """Pages for the attention layers of a model, handed out to sequences: per layer k, v
+    [n_pages, n_kv_heads, page, head_dim] in bf16 or float8_e4m3fn.  A page id means the same page in every
+    layer, so a sequence has one table for all of them.  k_scale, v_scale (f32 [layers, n_kv_heads],
+    float8_e4m3fn only): what a stored value is multiplied by; ones by default."""
+
+    def __init__(self, layers: int, n_pages: int, n_kv_heads: int, head_dim: int, page: int = 64, *,
+                 dtype: torch.dtype = torch.bfloat16, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None, device="cuda"):
+        if dtype not in _KV_TYPES:
+            raise ValueError("pages are bfloat16 or float8_e4m3fn")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+        if min(layers, n_pages, n_kv_heads, page) < 1:
+            raise ValueError("layers, n_pages, n_kv_heads and page must be at least 1")
+        if dtype == torch.bfloat16 and (k_scale is not None or v_scale is not None):
+            raise ValueError("scales are for float8_e4m3fn pages")
+        self.page, self.n_pages, self.dtype = page, n_pages, dtype
+        shape = (layers, n_pages, n_kv_heads, page, head_dim)
+        self.k, self.v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        self.k_scale = self.v_scale = [None] * layers
+        if dtype == torch.float8_e4m3fn:
+            one = lambda s: torch.ones(layers, n_kv_heads, device=device) if s is None else s
+            self.k_scale, self.v_scale = (list(one(s).to(device, torch.float32).contiguous()) for s in (k_scale, v_scale))
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def take(self, n: int) -> list[int]:
+        """n pages of nobody; raises when there are not as many."""
+        if n > len(self._free):
+            raise RuntimeError(f"the page pool is exhausted: {n} pages wanted, {len(self._free)} of {self.n_pages} free")
+        return [self._free.pop() for _ in range(n)]
+
+    def give(self, pages: list[int]) -> None:
+        self._free.extend(pages)
+
+
+class PageTable:
+    """One sequence's pages of a pool: the host list, and the row of the device table that the kernels read."""
+
+    def __init__(self, pool: PagePool, max_len: int):
+        self.pool, self.pages = pool, []
+        self.width = -(-max_len // pool.page)
+        self.device = torch.full((1, max(self.width, 1)), -1, dtype=torch.int32, device=pool.k.device)
+
+    def reserve(self, length: int) -> None:
+        """Pages for the first `length` positions (those that are there stay)."""
+        need = -(-length // self.pool.page)
+        if need > self.width:
+            raise ValueError(f"{length} positions do not fit a cache of {self.width * self.pool.page}")
+        n = len(self.pages)
+        if need > n:
+            self.pages += self.pool.take(need - n)
+            self.device[0, n:need] = torch.tensor(self.pages[n:], dtype=torch.int32).to(self.device.device, non_blocking=True)
+
+    def release(self) -> None:
+        """Every page back to the pool (also when the table is dropped)."""
+        self.pool.give(self.pages)
+        self.pages = []
+
+    def __del__(self):
+        if getattr(self, "pages", None):
+            self.release()
+
+
 def device_errors(device: torch.device | None = None, clear: bool = False) -> int:
     """The error bits of the paged calls made on `device` so far (synchronises with the current stream):
     0, or bit 9 for a sequence or page id out of range (skinny_b200.h).  clear: reset them afterwards."""
@@ -213,4 +281,4 @@ def device_errors(device: torch.device | None = None, clear: bool = False) -> in
     return word.value
 
 
-__all__ = ["append", "attention", "device_errors", "HEAD_DIMS", "MAX_BATCH", "MAX_TOKENS"]
+__all__ = ["append", "attention", "device_errors", "PagePool", "PageTable", "HEAD_DIMS", "MAX_BATCH", "MAX_TOKENS"]

@@ -8,10 +8,12 @@ loop -- with one kernel launch and a read-back of K+2 int32 values.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
+from .logprobs import TokenLogprobs, token_logprobs
 
 _ws: dict[tuple[int, int], torch.Tensor] = {}
 
@@ -105,6 +107,33 @@ def _accept_any(logits: torch.Tensor, draft: torch.Tensor) -> tuple[int, list[in
     while n < len(d) and d[n] == pred[n]:
         n += 1
     return n, d[:n] + [pred[n]]
+
+
+class TokenLogprob(NamedTuple):
+    """What the model thought of one emitted token: ln p of it, the entropy of its distribution (nats), and the
+    most likely tokens as (id, ln p), the likeliest first."""
+
+    logprob: float
+    entropy: float
+    top: list[tuple[int, float]]
+
+
+def _logprobs_any(logits: torch.Tensor, tokens: torch.Tensor, top_n: int):
+    """token_logprobs, or the same in torch (CPU runs of the model in tests)."""
+    if logits.is_cuda:
+        return token_logprobs(logits, tokens, top_n)
+    y = torch.log_softmax(logits.float(), -1)
+    order = torch.sort(logits.float(), dim=-1, descending=True, stable=True).indices[:, :top_n]
+    return TokenLogprobs(y.gather(1, tokens.long()[:, None])[:, 0], -torch.special.xlogy(y.exp(), y.exp()).sum(-1),
+                         y.gather(1, order), order.to(torch.int32))
+
+
+def _read_logprobs(parts: list) -> list[TokenLogprob]:
+    """The device results of a loop's steps on the host, one entry per token."""
+    if not parts:
+        return []
+    lp, ent, top, ids = (torch.cat(x).cpu().tolist() for x in zip(*parts))
+    return [TokenLogprob(a, b, list(zip(i, t))) for a, b, t, i in zip(lp, ent, top, ids)]
 
 
 class HybridRollback:
@@ -477,11 +506,14 @@ def _fresh_cache(model, cache):
     return cache
 
 
-def greedy(model, prompt: list[int], max_tokens: int, gaps: list | None = None, cache=None) -> list[int]:
+def greedy(model, prompt: list[int], max_tokens: int, gaps: list | None = None, cache=None,
+           logprobs: list | None = None, top_n: int = 0) -> list[int]:
     """Plain greedy decoding, one token per forward (skinny_mlx/spec.py:98-107).  `gaps`, when
     given, receives each step's (top1 - top2 logit gap, top1 logit), for the near-tie check.
-    `cache` (optional) is reset and reused, e.g. to keep a graph-replayed step's buffers."""
+    `cache` (optional) is reset and reused, e.g. to keep a graph-replayed step's buffers.  `logprobs`, when
+    given, receives one TokenLogprob per emitted token with its top_n alternatives (read back at the end)."""
     cache = _fresh_cache(model, cache)
+    scored = []
     _, logits = model(torch.tensor(prompt, device=model.device), cache)
     toks = []
     last = logits[-1]
@@ -493,23 +525,30 @@ def greedy(model, prompt: list[int], max_tokens: int, gaps: list | None = None, 
         # token (argmax returns the first maximal index, as the reference's does)
         y = torch.argmax(last).view(1)
         toks.append(y)
+        if logprobs is not None:
+            scored.append(_logprobs_any(last[None], y, top_n))
         if i + 1 == max_tokens:
             break
         _, logits = model(y, cache)
         last = logits[-1]
+    if logprobs is not None:
+        logprobs += _read_logprobs(scored)
     return torch.cat(toks).tolist()
 
 
 def speculative(model, prompt: list[int], max_tokens: int, drafter, k: int, stats: dict | None = None,
-                cache=None) -> list[int]:
+                cache=None, logprobs: list | None = None, top_n: int = 0) -> list[int]:
     """Greedy-exact speculative decoding (skinny_mlx/spec.py:110-156): each step verifies
     [last token] + K drafts in one forward (M = K+1), accepts the longest matching prefix on the
     device, emits one bonus token and rolls the hybrid cache back to the accepted prefix.
-    `cache` (optional) is reset and reused."""
+    `cache` (optional) is reset and reused.  `logprobs` and top_n as for greedy (the verified rows' own)."""
     cache = _fresh_cache(model, cache)
     rb = HybridRollback()
     h, logits = model(torch.tensor(prompt, device=model.device), cache)
     out = [int(torch.argmax(logits[-1].float()))]
+    scored = []
+    if logprobs is not None:
+        scored.append(_logprobs_any(logits[-1:], torch.tensor(out, device=model.device), top_n))
     drafter.begin(prompt, h, out[0])
     steps = accepted = 0
     while len(out) < max_tokens:
@@ -518,6 +557,8 @@ def speculative(model, prompt: list[int], max_tokens: int, drafter, k: int, stat
         rb.record(cache)
         h, logits = model(x.long(), cache)
         n, new = _accept_any(logits, draft)
+        if logprobs is not None:
+            scored.append(_logprobs_any(logits[:n + 1], torch.tensor(new, device=model.device), top_n))
         rb.rollback(cache, fed=x.numel(), keep=n + 1)
         drafter.update(h[: n + 1], new)
         out += new
@@ -525,6 +566,8 @@ def speculative(model, prompt: list[int], max_tokens: int, drafter, k: int, stat
         accepted += n
     if stats is not None:
         stats.update(steps=steps, tokens_per_step=len(out) / max(steps, 1), accepted=accepted)
+    if logprobs is not None:
+        logprobs += _read_logprobs(scored)[:max_tokens]
     return out[:max_tokens]
 
 
@@ -558,5 +601,5 @@ def speculative_tree(model, prompt: list[int], max_tokens: int, drafter, k: int,
     return out[:max_tokens]
 
 
-__all__ += ["HybridRollback", "MTPDrafter", "GraphedMTPDrafter", "PromptLookupDrafter", "ScriptedDrafter",
+__all__ += ["TokenLogprob", "HybridRollback", "MTPDrafter", "GraphedMTPDrafter", "PromptLookupDrafter", "ScriptedDrafter",
             "ScriptedTreeDrafter", "chain_tree", "greedy", "speculative", "speculative_tree"]

@@ -1,0 +1,251 @@
+"""Paged caches under the models and the decode loops, and the loops' token log probabilities."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import logprobs as olp
+from oracle.checks import argmax_violations, rel_err
+from skinny_mlx_b200.dense import DenseModel, small_dense
+from skinny_mlx_b200.model import SMALL, HybridModel, PagedAttnCache
+from skinny_mlx_b200.paged import PagePool, PageTable
+from skinny_mlx_b200.spec import HybridRollback, ScriptedDrafter, greedy, speculative
+
+PROMPT = [int(x) for x in np.random.default_rng(5).integers(0, SMALL.vocab, 24)]
+F8 = torch.float8_e4m3fn
+
+
+def _pool(model, n_pages=40, page=7, **kw):
+    return model.make_pool(n_pages, page, **kw)
+
+
+@pytest.fixture(scope="module")
+def cpu_model():
+    return HybridModel(SMALL, seed=0, device="cpu")
+
+
+def test_pool_and_table_bookkeeping():
+    pool = PagePool(2, 5, 2, 64, 4, device="cpu")
+    a, b = PageTable(pool, 16), PageTable(pool, 9)
+    assert (a.width, b.width, pool.free_pages) == (4, 3, 5)
+    a.reserve(5)
+    b.reserve(9)
+    assert len(a.pages) == 2 and len(b.pages) == 3 and pool.free_pages == 0
+    assert sorted(a.pages + b.pages) == list(range(5))
+    assert a.device[0].tolist() == a.pages + [-1, -1]
+    a.reserve(8)  # (the pages are there)
+    with pytest.raises(RuntimeError, match="exhausted"):
+        a.reserve(9)
+    with pytest.raises(ValueError, match="fit"):
+        b.reserve(13)
+    b.release()
+    a.reserve(16)
+    assert len(a.pages) == 4 and pool.free_pages == 1
+    for bad in (dict(dtype=torch.float16), dict(head_dim=96), dict(n_pages=0), dict(k_scale=torch.ones(2, 2))):
+        with pytest.raises(ValueError):
+            PagePool(**{**dict(layers=2, n_pages=5, n_kv_heads=2, head_dim=64, page=4, device="cpu"), **bad})
+
+
+def test_caches_refuse_foreign_pools_and_trees(cpu_model):
+    with pytest.raises(ValueError, match="pool"):
+        cpu_model.make_cache(pool=PagePool(2, 5, 2, 128, 4, device="cpu"))
+    with pytest.raises(ValueError, match="pool"):
+        DenseModel(small_dense(), seed=3, device="cpu").make_cache(pool=PagePool(2, 5, 2, 128, 4, device="cpu"))
+    c = cpu_model.make_cache(pool=_pool(cpu_model))
+    cpu_model(torch.tensor(PROMPT), c)
+    HybridRollback().record(c)
+    with pytest.raises(ValueError, match="contiguous"):
+        cpu_model(torch.tensor([1, 2, 3]), c, tree=[-1, 0, 0])
+
+
+def test_cpu_decoding_on_pages_is_the_contiguous_one(cpu_model):
+    """The CPU path gathers the pages and computes what the contiguous cache computes: the same bits."""
+    m = cpu_model
+    ref = greedy(m, PROMPT, 12)
+    pool = _pool(m)
+    got = greedy(m, PROMPT, 12, cache=m.make_cache(pool=pool))
+    assert got == ref
+    cache = m.make_cache(pool=pool)
+    assert speculative(m, PROMPT, 12, ScriptedDrafter(ref, 0.7, SMALL.vocab, "cpu"), 3, cache=cache) == ref
+    used = pool.n_pages - pool.free_pages
+    cache.release()
+    assert pool.free_pages > pool.n_pages - used and all(c.length == 0 for c in cache.layers if isinstance(c, PagedAttnCache))
+
+
+def test_cpu_loops_report_log_probabilities(cpu_model):
+    m = cpu_model
+    lps, lps2 = [], []
+    ref = greedy(m, PROMPT, 8, logprobs=lps, top_n=3)
+    assert speculative(m, PROMPT, 8, ScriptedDrafter(ref, 0.7, SMALL.vocab, "cpu"), 3, logprobs=lps2, top_n=3) == ref
+    assert len(lps) == len(lps2) == 8
+    cache = m.make_cache()
+    _, logits = m(torch.tensor(PROMPT + ref[:-1]), cache)
+    lp, ent, top, ids, _ = olp.token_logprobs(logits[len(PROMPT) - 1:].float().numpy(), ref, 3)
+    for i, r in enumerate(lps):  # (one token at a time against all at once: bf16 logits a few steps apart)
+        assert abs(r.logprob - lp[i]) < 0.2 and abs(r.entropy - ent[i]) < 0.2
+        assert r.top[0][0] == ref[i] and math.isclose(r.top[0][1], r.logprob)
+        assert [t[1] for t in r.top] == sorted((t[1] for t in r.top), reverse=True)
+
+
+# ---------------------------------------------------------------------------------------------
+# on the GPU
+# ---------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def gpu_model(cuda_lib):
+    from skinny_mlx_b200.patch import patch_model
+
+    m = HybridModel(SMALL, seed=0, device="cuda")
+    patch_model(m)
+    return m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 7, 16, 64])
+def test_verify_steps_on_pages(gpu_model, dev, page):
+    """Prompt, single tokens, 8- and 16-token verify steps with rollbacks: the logits of the paged cache stay
+    within the verify path's bar (1.5e-2 of the largest logit, the same argmax but for near-ties) of the
+    contiguous one's."""
+    m = gpu_model
+    caches = [m.make_cache(256), m.make_cache(256, pool=m.make_pool(300 // page + 2, page))]
+    rng = np.random.default_rng(page)
+    ids = rng.integers(0, SMALL.vocab, 120).tolist()
+    at = 0
+    for T, keep in ((40, 40), (1, 1), (8, 3), (16, 16), (1, 1), (5, 1), (17, 17), (2, 2)):
+        x = torch.tensor(ids[at:at + T], device=dev)
+        out = []
+        for c in caches:
+            rb = HybridRollback()
+            rec = 1 < T <= 16
+            if rec:
+                rb.record(c)
+            out.append(m(x, c)[1].float().cpu().numpy())
+            if rec:
+                rb.rollback(c, fed=T, keep=keep)
+        assert rel_err(out[0], out[1]) <= 1.5e-2
+        assert not argmax_violations(out[0], out[1])
+        at += keep
+        assert caches[0].offset == caches[1].offset == at
+
+
+@pytest.mark.gpu
+def test_two_sequences_share_a_pool(gpu_model, dev):
+    """Interleaved decoding of two prompts on one pool gives each its own greedy tokens; a released sequence's
+    pages serve the next one."""
+    m = gpu_model
+    pool = m.make_pool(14, 16)
+    prompts = [PROMPT, PROMPT[::-1] + PROMPT[:9]]
+    want = [greedy(m, p, 10, cache=m.make_cache(pool=pool)) for p in prompts[:1]]
+    assert pool.free_pages == 14  # (a dropped cache gives its pages back)
+    caches = [m.make_cache(112, pool=pool) for _ in prompts]
+    toks, last = [[], []], []
+    for p, c in zip(prompts, caches):
+        last.append(m(torch.tensor(p, device=dev), c)[1][-1])
+    for _ in range(10):
+        for i, c in enumerate(caches):
+            y = torch.argmax(last[i]).view(1)
+            toks[i].append(int(y))
+            last[i] = m(y, c)[1][-1]
+    assert toks[0] == want[0]
+    free = pool.free_pages
+    caches[0].release()
+    assert pool.free_pages == free + 3  # 34 positions in pages of 16
+    again = greedy(m, prompts[1], 10, cache=m.make_cache(112, pool=pool))
+    assert again == toks[1]
+    for c in caches:
+        c.release()
+    with pytest.raises(RuntimeError, match="exhausted"):
+        m(torch.tensor(PROMPT * 10, device=dev), m.make_cache(pool=pool))
+
+
+@pytest.mark.gpu
+def test_eight_bit_pages(gpu_model, dev):
+    """e4m3 pages: the step runs and its logits stay near the bf16 cache's (keys and values carry 2^-4 of
+    themselves at most, averaged over the context: a tenth of the largest logit bounds it loosely)."""
+    m = gpu_model
+    x = torch.tensor(PROMPT, device=dev)
+    out = []
+    for pool in (m.make_pool(20, 16), m.make_pool(20, 16, dtype=F8), m.make_pool(
+            20, 16, dtype=F8, k_scale=torch.full((1, 2), 0.05), v_scale=torch.full((1, 2), 0.02))):
+        c = m.make_cache(256, pool=pool)
+        m(x, c)
+        out.append(m(x[:6], c)[1].float().cpu().numpy())
+    assert all(np.isfinite(o).all() and rel_err(out[0], o) < 0.1 for o in out)
+
+
+@pytest.mark.gpu
+def test_fused_steps_refuse_paged_caches(gpu_model, dev):
+    from skinny_mlx_b200.fused import FusedStep, GraphedStep
+
+    step = FusedStep(gpu_model)
+    c = gpu_model.make_cache(pool=gpu_model.make_pool(20, 16))
+    for s in (step, GraphedStep(step)):
+        with pytest.raises(ValueError, match="contiguous"):
+            s(torch.tensor([1, 2], device=dev), c)
+
+
+@pytest.mark.gpu
+def test_dense_model_on_pages(cuda_lib, dev):
+    m = DenseModel(small_dense(), seed=3, device=dev)
+    pool = PagePool(2, 20, 8, 128, 16, device=dev)
+    caches = [m.make_cache(128), m.make_cache(128, pool=pool)]
+    rng = np.random.default_rng(1)
+    for T in (30, 1, 8, 16):
+        x = torch.tensor(rng.integers(0, 4096, T), device=dev)
+        a, b = (m(x, c).float().cpu().numpy() for c in caches)
+        assert rel_err(a, b) <= 1.5e-2 and not argmax_violations(a, b)
+    assert caches[1][0].length == 55 and pool.free_pages == 16
+    caches[1][0].table.release()
+    assert pool.free_pages == 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fused", [False, True])
+def test_loops_report_log_probabilities(gpu_model, dev, fused):
+    """The reported values are the f64 oracle's on the very logits of the step (the model is wrapped to keep
+    them), for the tokens that were emitted."""
+    from skinny_mlx_b200.fused import FusedStep, GraphedStep
+
+    m = GraphedStep(FusedStep(gpu_model)) if fused else gpu_model
+
+    class Keep:
+        def __init__(self):
+            self.seen = []
+
+        def __getattr__(self, name):
+            return getattr(m, name)
+
+        def __call__(self, ids, cache):
+            h, logits = m(ids, cache)
+            self.seen.append(logits.float().cpu().numpy())
+            return h, logits
+
+    k, lps = Keep(), []
+    ref = greedy(k, PROMPT, 9, logprobs=lps, top_n=4)
+    rows = np.stack([s[-1] for s in k.seen[:9]])
+    _check(lps, rows, ref)
+    k, lps, stats = Keep(), [], {}
+    got = speculative(k, PROMPT, 9, ScriptedDrafter(ref, 0.6, SMALL.vocab, dev), 3, stats=stats, logprobs=lps, top_n=4)
+    assert len(lps) == 9
+    # a step's emitted tokens are the argmaxes of its first rows: walk the steps with the drafter's luck
+    rows, drafter = [k.seen[0][-1]], ScriptedDrafter(ref, 0.6, SMALL.vocab, "cpu")
+    drafter.begin(PROMPT, None, got[0])
+    for s in k.seen[1:]:
+        draft, n = drafter.draft(3).tolist(), 0
+        while n < 3 and draft[n] == int(np.argmax(s[n])):
+            n += 1
+        rows += list(s[:n + 1])
+        drafter.update(None, [0] * (n + 1))
+    assert len(rows) >= 9 and [int(np.argmax(r)) for r in rows[:9]] == got
+    _check(lps, np.stack(rows[:9]), got)
+
+
+def _check(lps, rows, tokens):
+    lp, ent, top, ids, spread = olp.token_logprobs(rows, tokens, 4)
+    for i, r in enumerate(lps):
+        # f32 sums of at most V / 256 + 64 terms in a chain, values rounded four times (as in the operator's test)
+        tol = (4096 / 256 + 68 + 2 * spread[i]) * 2.0 ** -24 + 4 * (2 * np.abs(rows[i]).max() + 9) * 2.0 ** -24
+        assert abs(r.logprob - lp[i]) <= tol and abs(r.entropy - ent[i]) <= tol * (2 + 4 * spread[i])
+        assert [t for t, _ in r.top] == ids[i].tolist()
+        assert all(abs(a - b) <= tol for (_, a), b in zip(r.top, top[i]))
