@@ -13,9 +13,9 @@
 //   the 8-column operand: S^T[key][row] = K q^T, then O^T[dim][row] += V^T P^T.  A decode step has
 //   few rows, so 8-column tiles waste the least of the matrix unit, and O needs D / 16 * 4 registers
 //   per 8 rows.
-// * Keys and values come by TMA, in boxes of up to 16 consecutive positions of a page (the largest
-//   power of two that divides the page size, so any page size works) x 128 bytes, swizzled, which
-//   makes the fragment loads below conflict-free.  The copy engine takes some 12 clocks per request
+// * Keys and values come by TMA, in boxes of up to a block's consecutive positions of a page (the
+//   largest power of two that divides the page size, so any page size works), in lines of 128 bytes,
+//   swizzled, which makes the fragment loads below conflict-free.  The copy engine takes some 12 clocks per request
 //   whatever its size: one request per 256-byte row held the kernel at 5.9 TB/s, per 128-byte row at
 //   3.1.  A warp copies its own blocks and waits for them alone (one mbarrier per stage of keys and of
 //   values): the loop has no CTA barrier.  Ordinary asynchronous copies (16 bytes per lane) stood in
@@ -64,14 +64,18 @@ struct PagedAttnPlan {
   int tile_log;    // keys of one tile, one block per warp (a power of two)
   int lead;        // what beginning an item costs, in tiles: counted on the line, so that the pieces balance
   int shift;       // log2 of the page size, or -1
-  int box;         // positions of one copy: the largest power of two up to 16 that divides the page size
+  int box;         // positions of one copy: the largest power of two, up to a block, that divides the page size
   int nchunk;      // row chunks of 8 NB rows, one per warp (1, 2 or 4); the other warps split keys
   int groups;      // row groups of nchunk chunks per kv head
+  int join_warps;  // warps per row of the join (a power of two up to 8)
   int rows;        // rows of one group: 8 NB nchunk
   int ctas;        // CTAs of the split launch
   long long* pre;  // [B + 1] where each sequence begins on the line
   float* ml;       // [2 ctas][rows][2] maximum (log2) and sum of a piece
   float* o;        // [2 ctas][rows][D]
+  uint32_t rep_inv; // ceil(2^32 / rep), 0 for rep = 1: r / rep of rows r < 2^16
+
+  __device__ __forceinline__ int token(int r) const { return rep_inv ? __umulhi(static_cast<uint32_t>(r), rep_inv) : r; }
 };
 
 // The positions some token of the sequence sees, and the tiles they make.
@@ -225,7 +229,6 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   if (tid == 0) gave_up = 0;
   fence_mbar_init();
   __syncthreads();
-  pdl_wait_prior_grid();
 
   // ---- this CTA's piece of the line: [u, u_end), beginning `off` units into sequence b
   int b;
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
 
   const int chunk = warp % plan.nchunk, slot = warp / plan.nchunk, slots = kPtWarps / plan.nchunk;
   const uint32_t kpr = static_cast<uint32_t>(p.kps / D), vpr = static_cast<uint32_t>(p.vps / D);
-  const int boxes = S::kKeys / plan.box, boxes_log = __ffs(boxes) - 1;  // copies of one line of a block
+  const int boxes = S::kKeys / plan.box;  // of one block
   uint8_t* const region = pt_smem + warp * S::kWarpBytes;
   float* const so = reinterpret_cast<float*>(region);                  // [8 NB][kORow], after the loop
   const uint32_t ring = smem_u32(region);                               // [stage][keys | values][line][key][kLine], swizzled
@@ -349,7 +352,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     // ---- the query rows, 8 dims per thread at a time: asked for before the keys and values
     constexpr int kQBatch = NB * D / 128 < 1 ? 1 : NB * D / 128;  // pieces per thread of one chunk
     const auto q_load = [&](int e) {
-      const int r = rbase + e / (D / 8), t = r / rep, h = kvh * rep + (r - t * rep);
+      const int r = rbase + e / (D / 8), t = plan.token(r), h = kvh * rep + (r - t * rep);
       return t < sp.cnt ? __ldg(reinterpret_cast<const uint4*>(p.q + cur * p.qs[0] + t * p.qs[1] + h * p.qs[2]) + e % (D / 8))
                         : make_uint4(0u, 0u, 0u, 0u);
     };
@@ -382,35 +385,51 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
       rv = static_cast<uint32_t>(pid) * vpr + in;
       return __ballot_sync(0xFFFFFFFFu, ok);
     };
-    // The block whose pages were looked up last (one key per lane) into stage st, one copy per lane; its
-    // slots have been read by all lanes.  what: 0 keys, 1 values, 2 both (on the keys' barrier).  A box
-    // without a key that exists is left out.
+    // The block whose pages were looked up last (one key per lane) into stage st, whose slots have been
+    // read.  what: 0 keys, 1 values, 2 both (on the keys' barrier).  A box without a key that exists is
+    // left out.
     const auto copy = [&](int st, int what, uint32_t exist) {
       const int bit = st * 2 + (what & 1);
-      const uint32_t bar = bar0 + bit * 8;
-      const uint32_t mask = (1u << plan.box) - 1u;
+      const uint32_t bar = bar0 + bit * 8, dst = ring + st * (2 * S::kKBytes);
+      pending |= 1u << bit;
+      if (boxes == 1) {  // one copy each, by lane 0
+        const int src = exist ? __ffs(exist) - 1 : 0;
+        const int row_k = static_cast<int>(__shfl_sync(0xFFFFFFFFu, rk, src)) - src;  // (orders the lanes' reads too)
+        const int row_v = static_cast<int>(__shfl_sync(0xFFFFFFFFu, rv, src)) - src;
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, exist ? S::kKBytes * (what == 2 ? 2 : 1) : 0);
+          if (exist) {
+            if (what != 1) tma_load_3d(dst, &kmap, 0, row_k, 0, bar);
+            if (what != 0) tma_load_3d(dst + S::kKBytes, &vmap, 0, row_v, 0, bar);
+          }
+        }
+        return;
+      }
+      const uint32_t mask = (1u << plan.box) - 1u;  // one box per lane
       const int some = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && (exist >> (lane * plan.box) & mask)));
       if (lane == 0) mbar_arrive_expect_tx(bar, some * plan.box * S::kRow * (what == 2 ? 2 : 1));
       __syncwarp();
-      const int n = (boxes << (what == 2 ? 1 : 0)) * S::kLines;
+      const int n = what == 2 ? 2 * boxes : boxes;
       for (int q0 = 0; q0 < n; q0 += 32) {
-        const int q = q0 + lane, first = (q & (boxes - 1)) * plan.box, rest = q >> boxes_log;
-        const int kv = what == 2 ? rest & 1 : what, line = what == 2 ? rest >> 1 : rest;
-        const uint32_t here = exist & mask << first;
+        const int q = q0 + lane, first = (q & (boxes - 1)) * plan.box, kv = what == 2 ? q >= boxes : what;
+        const uint32_t here = q < n ? exist & mask << first : 0u;
         const int src = here ? __ffs(here) - 1 : 0;
         const uint32_t row_k = __shfl_sync(0xFFFFFFFFu, rk, src), row_v = __shfl_sync(0xFFFFFFFFu, rv, src);
         const uint32_t row = (kv ? row_v : row_k) - static_cast<uint32_t>(src - first);
-        if (q < n && here) {
-          const uint32_t dst = ring + (st * 2 + kv) * S::kKBytes + (line * S::kKeys + first) * S::kLine;
+        const uint32_t to = dst + kv * S::kKBytes + first * S::kLine;
+        if (here) {
           if (S::kLine == 64 && plan.box == 1) {  // 64 bytes: less than a tiled copy's alignment
             const uint8_t* const from = static_cast<const uint8_t*>(kv ? p.vp : p.kp) + static_cast<size_t>(row) * S::kRow;
-            for (int c = 0; c < 4; ++c) bulk_g2s(dst + ((c ^ (first >> 1 & 3)) << 4), from + 16 * c, 16, bar);
+            for (int c = 0; c < 4; ++c) bulk_g2s(to + ((c ^ (first >> 1 & 3)) << 4), from + 16 * c, 16, bar);
           } else {
-            tma_load_2d(dst, kv ? &vmap : &kmap, line * (S::kLine / S::kEs), static_cast<int>(row), bar);
+            // (a box of several lines would lay them out box by box: one line each)
+#pragma unroll
+            for (int c = 0; c < S::kLines; ++c)
+              tma_load_3d(to + c * (S::kKeys * S::kLine), kv ? &vmap : &kmap, 0, static_cast<int>(row), c, bar);
           }
         }
       }
-      pending |= 1u << bit;
     };
     const auto arrived = [&](int bit) {  // bounded; the same answer in every lane
       const bool ok = mbar_wait(bar0 + bit * 8, parity >> bit & 1u, p.seq.err, kErrBitWaitFull, &gave_up);
@@ -505,7 +524,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     uint32_t tokens = 0;
     if (p.seq.T > 1) {
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) tokens |= min(15, (r0 + 8 * (i >> 1) + 2 * cq + (i & 1)) / rep) << (4 * i);
+      for (int i = 0; i < 2 * NB; ++i) tokens |= min(15, plan.token(r0 + 8 * (i >> 1) + 2 * cq + (i & 1))) << (4 * i);
     }
 
     // ---- one pass over the blocks
@@ -782,7 +801,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
             if (!isfinite(v))
 #pragma unroll 1
               for (int r = 0; r < 8 * NB; ++r)
-                if (sees((r0 + r) / rep, j)) so[r * S::kORow + d] += v;
+                if (sees(plan.token(r0 + r), j)) so[r * S::kORow + d] += v;
           }
         }
       }
@@ -808,7 +827,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
           sum = fmaf(f[w], sml[c + w * plan.nchunk][rr][1], sum);
         }
       }
-      const int t = (rbase + r) / rep, h = kvh * rep + (rbase + r - t * rep);
+      const int t = plan.token(rbase + r), h = kvh * rep + (rbase + r - t * rep);
       out_row = (cur * p.seq.T + t) * p.Hq + h;
       inv = sum == 0.f ? 0.f : (F8 ? p.v_scale[kvh] : 1.f) / sum;
       if (warp + kPtWarps * lane < live) {
@@ -850,9 +869,9 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.seq.err, kErrBitBadInput);
 }
 
-// Joins the pieces of the items that were split, one output row per CTA, and writes the rows that no
-// piece covers (idle slots, padding).  Warp w adds pieces w, w + 8, ... and the results are added in
-// order.
+// Joins the pieces of the items that were split and writes the rows that no piece covers (idle slots,
+// padding).  plan.join_warps warps per output row: warp w of them adds pieces w, w + join_warps, ... and
+// the results are added in order.
 constexpr int kPtJoinWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(32 * kPtJoinWarps)
@@ -860,36 +879,45 @@ __global__ void __launch_bounds__(32 * kPtJoinWarps)
   constexpr int kPer = D / 32;
   constexpr int kAhead = 4;  // pieces whose loads are issued together
   __shared__ float so[kPtJoinWarps][D], sml[kPtJoinWarps][2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, W = plan.join_warps, sub = warp & (W - 1);
   const int rep = p.Hq / p.Hkv;
-  const int row = blockIdx.x, bt = row / p.Hq, h = row - bt * p.Hq, b = bt / p.seq.T, t = bt - b * p.seq.T;
+  const int rows = p.seq.B * p.seq.T * p.Hq, row = blockIdx.x * (kPtJoinWarps / W) + warp / W;
+  const int bt = row / p.Hq, h = row - bt * p.Hq, b = bt / p.seq.T, t = bt - b * p.seq.T;
   const int kvh = h / rep, r = t * rep + (h - kvh * rep), group = r / plan.rows, rr = r - group * plan.rows;
   const int item = kvh * plan.groups + group;
   pdl_launch_dependents();
   pdl_wait_prior_grid();
-  const long long begins = __ldcg(plan.pre + b), total = __ldcg(plan.pre + p.seq.B);
-  const PagedSpan sp = paged_span(p, plan, b);
-  if (t >= sp.cnt) {  // padding
-    if (tid < D / 8) reinterpret_cast<uint4*>(p.out + static_cast<size_t>(row) * D)[tid] = make_uint4(0u, 0u, 0u, 0u);
-    if (tid == 0 && p.lse) p.lse[row] = -INFINITY;
-    return;
+  int first = 0, last = -1;  // the pieces' CTAs
+  bool join = false;
+  long long beg = 0;
+  PtLine line(0, plan.ctas);
+  if (row < rows) {
+    const long long begins = __ldcg(plan.pre + b), total = __ldcg(plan.pre + p.seq.B);
+    const PagedSpan sp = paged_span(p, plan, b);
+    if (t >= sp.cnt) {  // padding
+      if (lane < D / 8 && sub == 0)
+        reinterpret_cast<uint4*>(p.out + static_cast<size_t>(row) * D)[lane] = make_uint4(0u, 0u, 0u, 0u);
+      if (lane == 0 && sub == 0 && p.lse) p.lse[row] = -INFINITY;
+    } else {
+      line = PtLine(total, plan.ctas);
+      beg = begins + static_cast<long long>(item) * sp.units;
+      first = line.owner(beg + plan.lead);
+      last = line.owner(beg + sp.units - 1);
+      join = first != last;  // (else one CTA had the whole item)
+    }
   }
-  const PtLine line(total, plan.ctas);
-  const long long beg = begins + static_cast<long long>(item) * sp.units;
-  const int first = line.owner(beg + plan.lead), last = line.owner(beg + sp.units - 1);
-  if (first == last) return;  // one CTA had the whole item
   const auto piece = [&](int i) {  // where CTA i put this item: in its first piece unless it began another before
     return 2 * static_cast<size_t>(i) + (line.start(i) < beg);
   };
   float m = kPtNothing, l = 0.f, acc[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int i0 = first + warp; i0 <= last; i0 += kPtJoinWarps * kAhead) {
+  for (int i0 = join ? first + sub : last + 1; i0 <= last; i0 += W * kAhead) {
     float2 ml[kAhead];
     float x[kAhead][kPer];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
-      const int i = i0 + a * kPtJoinWarps;
+      const int i = i0 + a * W;
       ml[a] = make_float2(kPtNothing, 0.f);
 #pragma unroll
       for (int q = 0; q < kPer; ++q) x[a][q] = 0.f;
@@ -916,28 +944,36 @@ __global__ void __launch_bounds__(32 * kPtJoinWarps)
       for (int q = 0; q < kPer; ++q) acc[q] = fmaf(w, x[a][q], acc[q]);
     }
   }
+  const float vs = p.v_scale ? p.v_scale[kvh] : 1.f;
+  if (W > 1) {
 #pragma unroll
-  for (int q = 0; q < kPer; ++q) so[warp][lane + 32 * q] = acc[q];
-  if (lane == 0) {
-    sml[warp][0] = m;
-    sml[warp][1] = l;
+    for (int q = 0; q < kPer; ++q) so[warp][lane + 32 * q] = acc[q];
+    if (lane == 0) {
+      sml[warp][0] = m;
+      sml[warp][1] = l;
+    }
+    __syncthreads();
+    if (sub != 0) return;
+    float mx = m;
+    for (int w = 1; w < W; ++w) mx = fmaxf(mx, sml[warp + w][0]);
+    const float f0 = pt_exp2(m - mx);
+    l *= f0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) acc[q] *= f0;
+    for (int w = 1; w < W; ++w) {
+      const float f = pt_exp2(sml[warp + w][0] - mx);
+      l = fmaf(f, sml[warp + w][1], l);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) acc[q] = fmaf(f, so[warp + w][lane + 32 * q], acc[q]);
+    }
+    m = mx;
   }
-  __syncthreads();
-  if (2 * tid >= D) return;
-  float mx = kPtNothing, sum = 0.f, a0 = 0.f, a1 = 0.f;
+  if (!join) return;
+  const float inv = l == 0.f ? 0.f : vs / l;
 #pragma unroll
-  for (int w = 0; w < kPtJoinWarps; ++w) mx = fmaxf(mx, sml[w][0]);
-#pragma unroll
-  for (int w = 0; w < kPtJoinWarps; ++w) {
-    const float f = pt_exp2(sml[w][0] - mx);
-    const float2 x = *reinterpret_cast<const float2*>(&so[w][2 * tid]);
-    sum = fmaf(f, sml[w][1], sum);
-    a0 = fmaf(f, x.x, a0);
-    a1 = fmaf(f, x.y, a1);
-  }
-  const float inv = sum == 0.f ? 0.f : (p.v_scale ? p.v_scale[kvh] : 1.f) / sum;
-  *reinterpret_cast<uint32_t*>(p.out + static_cast<size_t>(row) * D + 2 * tid) = pt_pack<false>(a0 * inv, a1 * inv);
-  if (tid == 0 && p.lse) p.lse[row] = (mx + log2f(sum)) * 0.6931471805599453f;
+  for (int q = 0; q < kPer; ++q)
+    p.out[static_cast<size_t>(row) * D + lane + 32 * q] = __float2bfloat16_rn(acc[q] * inv);
+  if (lane == 0 && p.lse) p.lse[row] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -978,10 +1014,10 @@ PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8) {
 
 size_t pt_round(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-// A pool as a matrix of its rows of D elements, to be read in boxes of `box` rows x `line` bytes.  The
-// pages of a pool that interleaves others are further apart: the rows between are never asked for.
+// A pool as [line of 128 bytes][row of D elements][element], to be read in boxes of `lines` lines x `box` rows.
+// The pages of a pool that interleaves others are further apart: the rows between are never asked for.
 cudaError_t pt_map(CUtensorMap* map, const void* pool, long long page_stride, const PagedAttnParams& p, int es, int line,
-                   int box) {
+                   int box, int lines) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -998,9 +1034,11 @@ cudaError_t pt_map(CUtensorMap* map, const void* pool, long long page_stride, co
   }
   const cuuint64_t rows = static_cast<cuuint64_t>(p.seq.n_pages - 1) * (page_stride / p.D) +
                           static_cast<cuuint64_t>(p.Hkv) * p.seq.page;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.D), rows}, strides[1] = {static_cast<cuuint64_t>(p.D) * es};
-  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(line / es), static_cast<cuuint32_t>(box)}, steps[2] = {1, 1};
-  const CUresult r = encode(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+  const cuuint32_t elems = static_cast<cuuint32_t>(line / es);
+  const cuuint64_t dims[3] = {elems, rows, static_cast<cuuint64_t>(p.D) / elems};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.D) * es, static_cast<cuuint64_t>(line)};
+  const cuuint32_t boxes[3] = {elems, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(lines)}, steps[3] = {1, 1, 1};
+  const CUresult r = encode(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                             const_cast<void*>(pool), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1019,10 +1057,14 @@ cudaError_t pt_split(const PagedAttnParams& p, const PagedAttnPlan& plan, int de
     attr_set[dev].store(true, std::memory_order_release);
   }
   CUtensorMap kmap, vmap;
-  cudaError_t e = pt_map(&kmap, p.kp, p.kps, p, S::kEs, S::kLine, plan.box);
-  if (e == cudaSuccess) e = pt_map(&vmap, p.vp, p.vps, p, S::kEs, S::kLine, plan.box);
+  const int lines = plan.box == S::kKeys ? S::kLines : 1;
+  cudaError_t e = pt_map(&kmap, p.kp, p.kps, p, S::kEs, S::kLine, plan.box, lines);
+  if (e == cudaSuccess) e = pt_map(&vmap, p.vp, p.vps, p, S::kEs, S::kLine, plan.box, lines);
   if (e != cudaSuccess) return e;
   cfg.dynamicSmemBytes = smem;
+  // Not a dependent launch: its CTAs would be placed around those of the kernel before, unevenly, for
+  // their whole run (long context 183 us, else 170).
+  cfg.numAttrs = 0;
   return cudaLaunchKernelEx(&cfg, kernel, p, plan, kmap, vmap);
 }
 
@@ -1037,7 +1079,8 @@ cudaError_t pt_launch(const PagedAttnParams& p, const PagedAttnPlan& plan, int n
     if (nb == 2 && f8) e = pt_split<D, 2, true>(p, plan, dev, cfg);
   }
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(p.seq.B) * p.seq.T * p.Hq));
+  const long long rows = static_cast<long long>(p.seq.B) * p.seq.T * p.Hq;
+  cfg.gridDim = dim3(static_cast<unsigned>((rows * plan.join_warps + kPtJoinWarps - 1) / kPtJoinWarps));
   cfg.blockDim = dim3(32 * kPtJoinWarps);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<D>, p, plan);
@@ -1067,8 +1110,14 @@ cudaError_t paged_attn_launch(const PagedAttnParams& p, bool f8, void* ws, int n
   plan.shift = -1;
   for (int i = 0; i < 31; ++i)
     if (p.seq.page == 1 << i) plan.shift = i;
-  plan.box = 16;
+  plan.box = 1 << (c.tile_log - 2);  // a block's keys
   while (p.seq.page % plan.box) plan.box /= 2;
+  const uint32_t rep = static_cast<uint32_t>(p.Hq / p.Hkv);
+  plan.rep_inv = rep == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + rep - 1) / rep);
+  // Few rows are split among many CTAs each: up to 8 warps per row while all are on the GPU at once.
+  const long long out_rows = static_cast<long long>(p.seq.B) * p.seq.T * p.Hq;
+  plan.join_warps = kPtJoinWarps;
+  while (plan.join_warps > 1 && out_rows * plan.join_warps > 32ll * n_sm) plan.join_warps /= 2;
   plan.nchunk = c.nchunk;
   plan.groups = c.groups;
   plan.rows = c.rows;
