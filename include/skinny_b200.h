@@ -408,7 +408,7 @@ size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D);
 /* Attention of the step's T <= 16 new tokens per sequence (already appended) over its pages:
  * out[b, t, h] (bf16, dense [B, T, Hq, D]) = softmax(scale * q . k_j) v over the positions
  * j <= lengths[b] + t, and j > lengths[b] + t - window when window > 0; query head h reads kv head
- * h / (Hq / Hkv).  lse (f32 [B, T, Hq], may be NULL) = ln sum_j exp(scale * q . k_j).  A row that
+ * h / (Hq / Hkv) (at most 1024 query heads each; B <= 8192; a pool holds fewer than 2^31 rows of D).  lse (f32 [B, T, Hq], may be NULL) = ln sum_j exp(scale * q . k_j).  A row that
  * sees no key has output 0 and lse -inf.  Keys a row does not see have no influence on it, whatever
  * they hold (infinities and NaN included). */
 int skinny_paged_attn(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -418,8 +418,9 @@ int skinny_paged_attn(const void* q, const long long* q_strides, const void* k_p
                       float* lse, int B, int T, int Hq, int Hkv, int D, void* workspace, size_t workspace_bytes,
                       void* stream);
 
-/* The current device's paged error word (0: none; sticky), copied as one uint32 to dst (may be NULL)
- * in stream order, then cleared when clear != 0. */
+/* The current device's paged error word (0: none; sticky; bit 9 as above, bit 0: a bounded wait inside
+ * skinny_paged_attn ran out and its outputs are void), copied as one uint32 to dst (may be NULL) in
+ * stream order, then cleared when clear != 0. */
 int skinny_paged_errors(void* dst, int clear, void* stream);
 
 /* Workspace bytes of skinny_token_logprobs (0 when the shape is not supported); scratch of one call,

@@ -642,7 +642,7 @@ int skinny_paged_append(const void* q, const long long* q_strides, const void* k
 
 size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D) {
   if (B < 1 || B > skinny::kPagedMaxBatch || T < 1 || T > skinny::kPagedMaxTokens || Hkv < 1 || Hkv > 1024 || Hq < 1 ||
-      Hq % Hkv || (D != 64 && D != 128 && D != 256))
+      Hq % Hkv || Hq / Hkv > skinny::kPagedMaxGroup || (D != 64 && D != 128 && D != 256))
     return 0;
   return skinny::paged_attn_ws_bytes(B, T, Hq, Hkv, D, skinny::device_sm_count(current_device()));
 }
@@ -660,7 +660,8 @@ int skinny_paged_attn(const void* q, const long long* q_strides, const void* k_p
   if (st != SKINNY_OK) return st;
   if (!out || window < 0) return SKINNY_ERR_INVALID_ARG;
   if (T < 1 || T > skinny::kPagedMaxTokens) return SKINNY_ERR_TOKENS;
-  if (Hq < 1 || Hq % Hkv || static_cast<long long>(B) * T * Hq > INT32_MAX) return SKINNY_ERR_SHAPE;
+  if (Hq < 1 || Hq % Hkv || Hq / Hkv > skinny::kPagedMaxGroup || static_cast<long long>(B) * T * Hq > INT32_MAX)
+    return SKINNY_ERR_SHAPE;
   // the copies' coordinate, a pool's row of D elements, is an int32
   if (n_pages > 0 && std::max(k_page_stride, v_page_stride) / D > INT32_MAX / n_pages) return SKINNY_ERR_SHAPE;
   if (!aligned16(out) || !aligned4(lse)) return SKINNY_ERR_ALIGNMENT;

@@ -20,6 +20,7 @@ namespace skinny {
 
 constexpr int kPagedMaxTokens = 16;    // new tokens per sequence of one attention call
 constexpr int kPagedMaxBatch = 8192;   // sequences per call
+constexpr int kPagedMaxGroup = 1024;   // query heads per kv head
 
 struct PagedSeqs {
   const int32_t* lengths;  // [B] tokens in the cache before the step

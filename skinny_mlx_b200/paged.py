@@ -176,8 +176,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, blo
     hq = q.shape[2]
     if t > MAX_TOKENS:
         raise ValueError(f"at most {MAX_TOKENS} new tokens per sequence")
-    if hq < 1 or hkv < 1 or hq % hkv:
-        raise ValueError(f"{hq} query heads do not divide over {hkv} kv heads")
+    if hq < 1 or hkv < 1 or hq % hkv or hq > 1024 * hkv:
+        raise ValueError(f"{hq} query heads do not divide over {hkv} kv heads, at most 1024 each")
     if window is not None and not 1 <= window < 2**31:
         raise ValueError("window must be at least 1")
     if scale is None:
@@ -272,7 +272,8 @@ class PageTable:
 
 def device_errors(device: torch.device | None = None, clear: bool = False) -> int:
     """The error bits of the paged calls made on `device` so far (synchronises with the current stream):
-    0, or bit 9 for a sequence or page id out of range (skinny_b200.h).  clear: reset them afterwards."""
+    0; bit 9: a sequence or page id out of range; bit 0: a bounded wait ran out, the outputs of that call are
+    void (skinny_b200.h).  clear: reset them afterwards."""
     word = ctypes.c_uint32()
     with torch.cuda.device(device):
         stream = torch.cuda.current_stream()

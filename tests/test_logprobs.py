@@ -155,6 +155,34 @@ def test_special_values(cuda_lib, dev, v, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("top", [0, 3])
+def test_more_rows_than_a_grid_holds(cuda_lib, dev, top):
+    torch.manual_seed(1)
+    x = torch.randn(70001, 24, device=dev)
+    _check(x, torch.randint(0, 24, (70001,), device=dev), top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [2, 450])
+def test_masked_vocabularies(cuda_lib, dev, rows, dtype):
+    """Rows of which a mask leaves one, a few, a run, or fewer tokens than alternatives asked for (in one part per
+    row and in several)."""
+    torch.manual_seed(rows)
+    v = 20000
+    x = (torch.randn(rows, v, device=dev) * 3).to(dtype)
+    keep = torch.zeros(rows, v, dtype=torch.bool, device=dev)
+    for r in range(rows):
+        n = (1, 7, 19, 20, 21, 300)[r % 6]
+        if r % 2:
+            keep[r, torch.randperm(v, device=dev)[:n]] = True
+        else:
+            keep[r, v - 1 - n:v - 1] = True
+    x.masked_fill_(~keep, -math.inf if rows == 2 else torch.finfo(dtype).min)
+    _check(x, torch.randint(0, v, (rows,), device=dev), 20)
+
+
+@pytest.mark.gpu
 def test_tokens_outside_the_vocabulary(cuda_lib, dev):
     x = torch.randn(6, 100, device=dev)
     tok = torch.tensor([-1, 100, 99, 0, 2**31 - 1, -2**31], device=dev)

@@ -79,7 +79,7 @@ def test_append_entry_refuses(kw, status):
 
 @pytest.mark.parametrize("kw,status", COMMON + [
     (dict(q=None), -1), (dict(out=None), -1), (dict(window=-1), -1), (dict(T=0), -3), (dict(T=17), -3), (dict(Hq=3), -2),
-    (dict(Hq=0), -2), (dict(n=1 << 30), -2), (dict(vps=1 << 40), -2), (dict(out=F + 8), -4), (dict(lse=F + 2), -4), (dict(ws=None), -5), (dict(wsn=0), -5), (dict(ws=F + 4), -5)])
+    (dict(Hq=0), -2), (dict(Hq=2 * 1025), -2), (dict(n=1 << 30), -2), (dict(vps=1 << 40), -2), (dict(out=F + 8), -4), (dict(lse=F + 2), -4), (dict(ws=None), -5), (dict(wsn=0), -5), (dict(ws=F + 4), -5)])
 def test_attention_entry_refuses(kw, status):
     assert _attn_status(**kw) == status
 
@@ -88,7 +88,8 @@ def test_workspace_of_unsupported_shapes_is_zero():
     from skinny_mlx_b200 import _lib
 
     ws = _lib.lib().skinny_paged_attn_workspace_bytes
-    for bad in ((0, 1, 4, 2, 128), (8193, 1, 4, 2, 128), (1, 17, 4, 2, 128), (1, 1, 4, 3, 128), (1, 1, 4, 2, 96), (1, 1, 0, 2, 64)):
+    for bad in ((0, 1, 4, 2, 128), (8193, 1, 4, 2, 128), (1, 17, 4, 2, 128), (1, 1, 4, 3, 128), (1, 1, 4, 2, 96), (1, 1, 0, 2, 64),
+                (1, 1, 2050, 2, 64)):
         assert ws(*bad) == 0
 
 
@@ -339,6 +340,68 @@ def test_attention_ragged_counts_scale_and_strides(cuda_lib, dev, kv):
 def test_attention_long_and_many(cuda_lib, dev, lengths, page, T, Hq, Hkv, kv):
     c = Case(dev, lengths, T=T, Hq=Hq, Hkv=Hkv, page=page, kv=kv, seed=len(lengths))
     check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("B", [33, 129, 700])
+def test_attention_batches_wider_than_a_warp_and_a_block(cuda_lib, dev, B, kv):
+    """More sequences than a warp, a CTA's threads, and several per thread; idle ones and empty ones among them."""
+    lengths = [(37 * i) % 150 if i % 7 else 0 for i in range(B)]
+    counts = [0 if i % 5 == 3 or i < 3 else 1 for i in range(B)]
+    c = Case(dev, lengths, counts, T=1, Hq=2, Hkv=1, D=64, page=8, kv=kv, seed=B)
+    check_attention(c.attend(), c.oracle(), c.D)
+    c.counts = torch.zeros_like(c.counts)
+    o, lse = c.attend()
+    assert (o == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page", [2, 3, 4, 8, 12, 16, 31, 32, 96, 1024])
+def test_attention_page_sizes(cuda_lib, dev, page, D, kv):
+    """Every size of copy a page allows, with windows that begin and lengths that end inside one."""
+    c = Case(dev, [0, 45, 262], T=3, Hq=6, Hkv=2, D=D, page=page, kv=kv, seed=page)
+    check_attention(c.attend(), c.oracle(), D)
+    check_attention(c.attend(window=37), c.oracle(window=37), D)
+
+
+@pytest.mark.gpu
+def test_pages_before_the_window_may_be_gone(cuda_lib, dev):
+    """Table entries of pages that no row sees are not looked at."""
+    from skinny_mlx_b200 import paged
+
+    c = Case(dev, [300, 97], T=2, Hq=4, Hkv=2, page=16, seed=1)
+    want = c.oracle(window=40)
+    c.table[0, :(300 + 1 - 40) // 16] = -1
+    c.table[1, :(97 + 1 - 40) // 16] = 10 ** 6
+    c.table[1, (97 + 2 + 15) // 16:] = -7
+    check_attention(c.attend(window=40), want, c.D)
+    assert paged.device_errors(dev, clear=True) == 0
+
+
+@pytest.mark.gpu
+def test_calls_from_two_threads(cuda_lib, dev):
+    """Two threads with streams of their own: every result is the one of a call alone."""
+    import threading
+
+    cases = [Case(dev, [500 + 300 * i, 40, 1200], T=1 + 3 * i, Hq=8, Hkv=2, page=16, seed=i) for i in range(2)]
+    want = [c.attend() for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(c, w):
+        with torch.cuda.stream(torch.cuda.Stream(dev)):
+            for _ in range(200):
+                got = c.attend()
+                if not all(torch.equal(a, b) for a, b in zip(got, w)):
+                    bad.append(1)
+
+    ts = [threading.Thread(target=work, args=a) for a in zip(cases, want)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
 
 
 @pytest.mark.gpu
