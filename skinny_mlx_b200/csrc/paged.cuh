@@ -51,6 +51,8 @@ struct PagedAppendParams {
   const float *k_scale, *v_scale;  // [Hkv] (8-bit pages)
   const float* inv_freq;
   int rot, Hq, Hkv, D;
+  uint32_t inv_per;                // (set by the launch) pieces per head: see the kernel
+  int perv_log;
 };
 
 struct PagedAttnParams {

@@ -28,7 +28,7 @@ namespace skinny {
 __device__ uint32_t g_paged_err;  // error bits of this device's paged calls
 
 constexpr int kPaThreads = 128;
-constexpr int kPaAhead = 2;      // pieces per thread whose loads are issued together (1: 46.8 us for 8191 tokens, 2: 44.5, 4: 53)
+constexpr int kPaAhead = 2;      // pieces per thread whose loads are issued together (1: 41.4 us for 8191 tokens, 2: 39.4, 4: 42.5)
 constexpr int kPaMaxHalf = 128;  // rotation pairs (head dim <= 256)
 
 __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
@@ -75,7 +75,8 @@ struct PagedPiece {
 
 template <bool F8>
 __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
-  __shared__ float2 cs[kPaMaxHalf];
+  // cos and sin of pair j at [j % 8][j / 8]: the lanes of a warp, at pairs 8 u + c, read neighbours
+  __shared__ float2 cs[8][kPaMaxHalf / 8];
   const int tid = threadIdx.x;
   const int b = blockIdx.x / p.seq.T, t = blockIdx.x % p.seq.T;
   const int half = p.rot >> 1;
@@ -88,19 +89,31 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const __grid_c
   const bool ok = p.seq.get(b, len, cnt);
   const bool live = t < cnt;
   const int pos = len + t;
+  // the token's rows; a piece's head by a multiplication (p.inv_per = ceil(2^32 / per), exact below 2^27 pieces)
+  const __nv_bfloat16* const qt = p.q + b * p.qs[0] + t * p.qs[1];
+  const __nv_bfloat16* const kt = p.k + b * p.ks[0] + t * p.ks[1];
+  const __nv_bfloat16* const vt = p.v + b * p.vs[0] + t * p.vs[1];
   const auto load = [&](int e) {
     PagedPiece q;
     q.kind = e >= all ? -1 : e < nq ? 0 : e < nq + nk ? 1 : 2;
-    const int r = e - (q.kind == 1 ? nq : q.kind == 2 ? nq + nk : 0), w = q.kind == 2 ? perv : per;
-    q.h = r / w;
-    const int u = r - q.h * w;
-    q.pair = q.kind != 2 && u < pairs;
-    q.d = q.kind == 2 || q.pair ? 8 * u : p.rot + 8 * (u - pairs);
+    int u;
+    if (q.kind == 2) {
+      q.h = (e - nq - nk) >> p.perv_log;
+      u = (e - nq - nk) & (perv - 1);
+      q.d = 8 * u;
+      q.pair = false;
+    } else {
+      const int r = q.kind == 1 ? e - nq : e;
+      q.h = p.inv_per ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), p.inv_per)) : r;
+      u = r - q.h * per;
+      q.pair = u < pairs;
+      q.d = q.pair ? 8 * u : p.rot + 8 * (u - pairs);
+    }
     q.x = q.y = make_uint4(0u, 0u, 0u, 0u);
     if (live && q.kind >= 0) {
-      const __nv_bfloat16* const src = (q.kind == 0   ? p.q + b * p.qs[0] + t * p.qs[1] + q.h * p.qs[2]
-                                        : q.kind == 1 ? p.k + b * p.ks[0] + t * p.ks[1] + q.h * p.ks[2]
-                                                      : p.v + b * p.vs[0] + t * p.vs[1] + q.h * p.vs[2]) + q.d;
+      const __nv_bfloat16* const src = (q.kind == 0   ? qt + q.h * p.qs[2]
+                                        : q.kind == 1 ? kt + q.h * p.ks[2]
+                                                      : vt + q.h * p.vs[2]) + q.d;
       q.x = *reinterpret_cast<const uint4*>(src);
       if (q.pair) q.y = *reinterpret_cast<const uint4*>(src + half);
     }
@@ -121,7 +134,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const __grid_c
       const double turns = static_cast<double>(pos) * static_cast<double>(p.inv_freq[j]) * 0.15915494309189533577;
       float sn, c;
       sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &c);
-      cs[j] = make_float2(c, sn);
+      cs[j & 7][j >> 3] = make_float2(c, sn);
     }
   }
   if (tid == 0 && blockIdx.y == 0 && (!ok || (live && page < 0))) atomicOr(p.seq.err, kErrBitBadInput);
@@ -139,7 +152,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const __grid_c
       if (q[i].pair && live) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          const float2 w = cs[q[i].d + c];
+          const float2 w = cs[c][q[i].d >> 3];
           const float a = x[c] * w.x - y[c] * w.y;
           y[c] = y[c] * w.x + x[c] * w.y;
           x[c] = a;
@@ -162,9 +175,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const __grid_c
   }
 }
 
-cudaError_t paged_append_launch(const PagedAppendParams& prm, bool f8, int n_sm, cudaStream_t stream) {
+cudaError_t paged_append_launch(const PagedAppendParams& params, bool f8, int n_sm, cudaStream_t stream) {
+  PagedAppendParams prm = params;
   const long long tokens = static_cast<long long>(prm.seq.B) * prm.seq.T;
   const int half = prm.rot / 2, per = half / 8 + (prm.D - prm.rot) / 8;
+  prm.inv_per = per == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + per - 1) / per);
+  prm.perv_log = prm.D == 64 ? 3 : prm.D == 128 ? 4 : 5;
   const int pieces = ((prm.q ? prm.Hq : 0) + prm.Hkv) * per + prm.Hkv * (prm.D / 8);
   // With few tokens their heads are spread over the SMs (each CTA then repeats the rotation table).
   const long long want = (2ll * n_sm + tokens - 1) / tokens;
