@@ -112,22 +112,32 @@ struct LpSums {
   }
 };
 
-// The same in the loop: M = fl(m log2(e)), sums of 2^y and 2^y y, y = x log2(e) - M, of bounded logits.
+// The same in the loop: M = fl(m log2(e)), sums of 2^y and 2^y y, y = x log2(e) - M, of bounded logits, in
+// two halves (even and odd logits).
 struct LpFast {
   float m = -2.f * kLpFar, M = -2.f * kLpFar * kLog2e;
-  LpSums a;
+  uint64_t z = 0, s = 0;  // pairs of f32
   __device__ __forceinline__ void renew(float n) {
     const float N = n * kLog2e;
+    LpSums a, b;
+    f2_unpack(z, a.z, b.z);
+    f2_unpack(s, a.s, b.s);
     a.scale(M - N, 1.f);
+    b.scale(M - N, 1.f);
+    z = f2_pack(a.z, b.z);
+    s = f2_pack(a.s, b.s);
     m = n;
     M = N;
   }
   __device__ __forceinline__ LpSums sums() const {
+    float z0, z1, s0, s1;
+    f2_unpack(z, z0, z1);
+    f2_unpack(s, s0, s1);
     const float r = fmaf(m, kLog2e, -M), f = lp_exp2(-r);  // 2^y = e^(x - m) 2^r
     LpSums b;
     b.m = m;
-    b.z = a.z * f;
-    b.s = f * fmaf(a.z, -r, a.s) * 0.6931471805599453f;
+    b.z = (z0 + z1) * f;
+    b.s = f * fmaf(z0 + z1, -r, s0 + s1) * 0.6931471805599453f;
     return b;
   }
 };
@@ -163,11 +173,8 @@ struct LpPiece {
       b.u[i] = F32 ? __float_as_uint(lp_max_nan(__uint_as_float(u[i]), kLpMasked)) : lp_max_nan2(u[i], kLpMasked2);
     return b;
   }
-  // A bounded piece with largest logit `top` to the sums.
-  __device__ __forceinline__ void add(LpFast& f, float top) const {
-    if (top > f.m) f.renew(top);
-    LpSums& a = f.a;
-    uint64_t z2 = f2_pack(0.f, 0.f), s2 = z2;
+  // A bounded piece to the sums (whose maximum it does not exceed).
+  __device__ __forceinline__ void add(LpFast& f) const {
     const uint64_t nm = f2_pack(-f.M, -f.M), one = f2_pack(1.f, 1.f), l2 = f2_pack(kLog2e, kLog2e);
 #pragma unroll
     for (int i = 0; i < kN; i += 2) {
@@ -175,14 +182,9 @@ struct LpPiece {
       const uint64_t y = f2_fma(f2_pack(at(i), at(i + 1)), l2, nm);
       f2_unpack(y, y0, y1);
       const uint64_t e = f2_pack(lp_exp2(y0), lp_exp2(y1));
-      z2 = f2_fma(e, one, z2);
-      s2 = f2_fma(e, y, s2);
+      f.z = f2_fma(e, one, f.z);
+      f.s = f2_fma(e, y, f.s);
     }
-    float a0, a1;
-    f2_unpack(z2, a0, a1);
-    a.z += a0 + a1;
-    f2_unpack(s2, a0, a1);
-    a.s += a0 + a1;
   }
 };
 
@@ -416,20 +418,53 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprob_part_kernel(const __gri
   float run_best[kLpRuns];  // the same of its pieces of each run
 #pragma unroll
   for (int u = 0; u < kLpRuns; ++u) run_best[u] = kLpMasked;
-  for (int base = 0; base < runs; base += kLpThreads) {
-    uint4 next[kLpRuns];
-    load(next, base + kLpThreads);  // in flight while this step's pieces are added
+  const auto step = [&](const uint4 (&v)[kLpRuns], int base) {
+    LpPiece<F32> b[kLpRuns] = {LpPiece<F32>(v[0]).bounded(), LpPiece<F32>(v[1]).bounded(), LpPiece<F32>(v[2]).bounded(),
+                               LpPiece<F32>(v[3]).bounded()};
+    float t[kLpRuns], most = kLpMasked;
 #pragma unroll
     for (int u = 0; u < kLpRuns; ++u) {
-      const LpPiece<F32> b = LpPiece<F32>(w[u]).bounded();
-      const float t = b.top();
-      if (TOP && t > best) {
-        best = t;
+      t[u] = b[u].top();
+      most = fmaxf(most, t[u]);
+      if (TOP && t[u] > best) {
+        best = t[u];
         best_at = u * runs + base + tid;
       }
-      if (TOP) run_best[u] = fmaxf(run_best[u], t);
-      b.add(fast, t);
+      if (TOP) run_best[u] = fmaxf(run_best[u], t[u]);
     }
+    if (most > fast.m) fast.renew(most);
+#pragma unroll
+    for (int u = 0; u < kLpRuns; ++u) b[u].add(fast);
+  };
+  // The next step's pieces are in flight while one's are added; then the steps that not every run fills.
+  // (Two steps per turn save the copies between the buffers but spill a little: 36 us against 39 for 509 rows
+  // with alternatives, 55 against 52 for 1024 without.)
+  static_assert(kLpRuns == 4, "step()");
+  uint4 next[kLpRuns];
+  const auto load_full = [&](uint4 (&v)[kLpRuns], int base) {
+#pragma unroll
+    for (int u = 0; u < kLpRuns; ++u) v[u] = __ldcs(body + u * runs + base + tid);
+  };
+  const int full = pieces - (kLpRuns - 1) * runs;  // pieces of the last run, the shortest
+  int base = 0;
+  if (TOP) {
+    for (; base + 3 * kLpThreads <= full; base += 2 * kLpThreads) {
+      load_full(next, base + kLpThreads);
+      step(w, base);
+      load_full(w, base + 2 * kLpThreads);
+      step(next, base + kLpThreads);
+    }
+  } else {
+    for (; base + 2 * kLpThreads <= full; base += kLpThreads) {
+      load_full(next, base + kLpThreads);
+      step(w, base);
+#pragma unroll
+      for (int u = 0; u < kLpRuns; ++u) w[u] = next[u];
+    }
+  }
+  for (; base < runs; base += kLpThreads) {
+    load(next, base + kLpThreads);
+    step(w, base);
 #pragma unroll
     for (int u = 0; u < kLpRuns; ++u) w[u] = next[u];
   }
@@ -556,7 +591,7 @@ __global__ void __launch_bounds__(kLpThreads) logprob_join_kernel(const __grid_c
 }
 
 // Parts per row.  From three rows per SM on a row is one CTA (509 rows with 20 alternatives: 42 us, in two
-// parts 45, in five 49: what a part and the join cost besides the logits); fewer rows are cut so that
+// parts 45, in five 49 before the last steps; now 36: what a part and the join cost besides the logits); fewer rows are cut so that
 // every SM has four CTAs (300 f32 rows: one part 54 us, two 48), of at least 4096 logits, and no more than the
 // join's list holds and its threads read.
 static void lp_parts(int rows, int V, int top, int n_sm, LpPlan& plan) {
