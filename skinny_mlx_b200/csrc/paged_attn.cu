@@ -560,13 +560,21 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
 #pragma unroll
         for (int sub = 0; sub < kSub; ++sub) s[nb][sub][0] = s[nb][sub][1] = s[nb][sub][2] = s[nb][sub][3] = 0.f;
       if (!arrived(stage * 2)) break;
+      // (fragments of 4 steps asked for together: verify 26.4 -> 25.2 us, of 8 the same)
+      constexpr int kSteps = S::kRow / 32, kBatch = kSteps < 4 ? kSteps : 4;
+      uint32_t kb[kBatch][kSub][4];
 #pragma unroll
-      for (int i = 0; i < S::kRow / 32; ++i) {  // 32 bytes of 16 (32) keys: one 16-dim step, or two of e4m3
-        uint32_t kw[kSub][4];
+      for (int i = 0; i < kSteps; ++i) {  // 32 bytes of 16 (32) keys: one 16-dim step, or two of e4m3
+        if (i % kBatch == 0)
 #pragma unroll
-        for (int sub = 0; sub < kSub; ++sub)
-          ldsm_x4((kaddr ^ (i * 32 % S::kLine)) + i * 32 / S::kLine * (S::kKeys * S::kLine) + sub * 16 * S::kLine, kw[sub][0],
-                  kw[sub][1], kw[sub][2], kw[sub][3]);
+          for (int a = 0; a < kBatch; ++a)
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub) {
+              uint32_t(&x)[4] = kb[a][sub];
+              ldsm_x4((kaddr ^ ((i + a) * 32 % S::kLine)) + (i + a) * 32 / S::kLine * (S::kKeys * S::kLine) + sub * 16 * S::kLine,
+                      x[0], x[1], x[2], x[3]);
+            }
+        uint32_t(&kw)[kSub][4] = kb[i % kBatch];
 #pragma unroll
         for (int c = 0; c < (F8 ? 2 : 1); ++c) {
           const int ks = F8 ? 2 * i + c : i;
@@ -845,17 +853,19 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
       const size_t row = __shfl_sync(0xFFFFFFFFu, out_row, i);
 #pragma unroll
       for (int d = 4 * lane; d < D; d += 128) {
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), x[kPtWarps];
 #pragma unroll
-        for (int w = 0; w < kPtWarps; ++w)
-          if (w < slots) {
-            const float4 x = *reinterpret_cast<const float4*>(pt_smem + (c + w * plan.nchunk) * S::kWarpBytes +
-                                                              (rr * S::kORow + d) * 4);
-            acc.x = fmaf(fr[w], x.x, acc.x);
-            acc.y = fmaf(fr[w], x.y, acc.y);
-            acc.z = fmaf(fr[w], x.z, acc.z);
-            acc.w = fmaf(fr[w], x.w, acc.w);
-          }
+        for (int w = 0; w < kPtWarps; ++w)  // (together: no branch between the loads)
+          x[w] = *reinterpret_cast<const float4*>(pt_smem + (w < slots ? c + w * plan.nchunk : c) * S::kWarpBytes +
+                                                  (rr * S::kORow + d) * 4);
+#pragma unroll
+        for (int w = 0; w < kPtWarps; ++w) {
+          const bool on = w < slots;  // (0 times an infinity is not 0)
+          acc.x = fmaf(fr[w], on ? x[w].x : 0.f, acc.x);
+          acc.y = fmaf(fr[w], on ? x[w].y : 0.f, acc.y);
+          acc.z = fmaf(fr[w], on ? x[w].z : 0.f, acc.z);
+          acc.w = fmaf(fr[w], on ? x[w].w : 0.f, acc.w);
+        }
         if (whole)
           *reinterpret_cast<uint2*>(p.out + row * D + d) =
               make_uint2(pt_pack<false>(acc.x * iv, acc.y * iv), pt_pack<false>(acc.z * iv, acc.w * iv));
