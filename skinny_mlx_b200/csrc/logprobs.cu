@@ -590,15 +590,20 @@ __global__ void __launch_bounds__(kLpThreads) logprob_join_kernel(const __grid_c
   }
 }
 
-// Parts per row.  From three rows per SM on a row is one CTA (509 rows with 20 alternatives: 42 us, in two
-// parts 45, in five 49 before the last steps; now 36: what a part and the join cost besides the logits); fewer rows are cut so that
-// every SM has four CTAs (300 f32 rows: one part 54 us, two 48), of at least 4096 logits, and no more than the
-// join's list holds and its threads read.
+// Parts per row.  Fewer than three rows per SM are cut so that every SM has four CTAs (300 f32 rows: one part
+// 54 us, two 48), into parts of at least 4096 logits, no more than the join's list holds and its threads
+// read.  From there on a row is one CTA (509 rows with 20 alternatives: one part 42 us, two 45, five 49: what a
+// part and the join cost besides the logits), except that without alternatives, where the join is cheap, rows
+// up to six per SM are cut into up to four parts of at least 32768 logits: whole rows, four to an SM, leave most
+// SMs idle at the end (760 rows of 152064 bf16 logits: one part 57 us, four 53; 600 f32 rows 82 and 70; at
+// 1024 rows 64 and 65, and 600 rows of 32000 logits 16 and 20).
 static void lp_parts(int rows, int V, int top, int n_sm, LpPlan& plan) {
   plan.cap = top > 0 ? top + 32 : 0;
   const int sms = std::max(n_sm, 1);
   const int most = std::min({V / 4096 + (V % 4096 > 0), kLpThreads, top > 0 ? kLpList / plan.cap : kLpThreads});
-  const int want = rows >= 3 * sms ? 1 : (4 * sms + rows - 1) / rows;
+  const int fill = rows >= 3 * sms ? 1 : (4 * sms + rows - 1) / rows;
+  const int even = top == 0 && rows < 6 * sms ? std::min(4, V / 32768) : 1;
+  const int want = std::max(fill, even);
   plan.parts = std::max(1, std::min(most, want));
   plan.part = ((V - 1) / plan.parts / 64 + 1) * 64;
   plan.parts = (V - 1) / plan.part + 1;

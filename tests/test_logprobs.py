@@ -94,6 +94,16 @@ def test_values(cuda_lib, dev, rows, v, top, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,v", [(450, 98309), (887, 65536)])
+def test_many_rows_of_a_large_vocabulary(cuda_lib, dev, rows, v):
+    torch.manual_seed(rows)
+    x = (torch.randn(rows, v, device=dev) * 3).bfloat16()
+    x[3, 40000:] = -math.inf  # (parts with nothing in them)
+    x[4, :60000] = -math.inf
+    _check(x, torch.randint(0, v, (rows,), device=dev, dtype=torch.int32), 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("off,ld", [(0, 1003), (1, 1001), (3, 1024), (7, 1000)])
 def test_strided_and_unaligned_rows(cuda_lib, dev, off, ld, dtype):
