@@ -547,6 +547,10 @@ class HybridModel(nn.Module):
     @torch.no_grad()
     def forward(self, ids: torch.Tensor, cache: Cache, tree=None):
         """tree: parents of the input tokens (a draft tree, see tree_paths), or None (a chain)."""
+        if cache.table is not None:  # what a paged cache refuses, before any layer's state has changed
+            if tree is not None:
+                raise ValueError("a tree verify needs a contiguous cache")
+            cache.table.reserve(cache.offset + ids.shape[0])
         x = self.embed_tokens(ids)
         for layer, c in zip(self.layers, cache.layers):
             x = layer(x, c, tree)

@@ -74,6 +74,27 @@ def test_cpu_decoding_on_pages_is_the_contiguous_one(cpu_model):
     assert pool.free_pages > pool.n_pages - used and all(c.length == 0 for c in cache.layers if isinstance(c, PagedAttnCache))
 
 
+def test_a_refused_step_changes_no_state(cpu_model):
+    """A step for which the pool has no pages, or a tree, is refused before the recurrent layers have taken it
+    in: when pages are there again the sequence goes on as if nothing had happened."""
+    m = cpu_model
+    x, y = torch.tensor(PROMPT), torch.tensor([5, 6, 7, 8])
+    c = m.make_cache()
+    m(x, c)
+    want = m(y, c)[1]
+    pool = m.make_pool(len(PROMPT) // 4 + 1, 4)
+    c, other = m.make_cache(pool=pool), m.make_cache(pool=pool)
+    m(x, c)  # (fills its pages)
+    other.table.reserve(4)
+    with pytest.raises(ValueError, match="contiguous"):
+        m(y, c, tree=[-1, 0, 1, 2])
+    with pytest.raises(RuntimeError, match="exhausted"):
+        m(y, c)
+    assert c.offset == len(PROMPT)
+    other.release()
+    assert torch.equal(m(y, c)[1], want)
+
+
 def test_cpu_loops_report_log_probabilities(cpu_model):
     m = cpu_model
     lps, lps2 = [], []
