@@ -370,7 +370,7 @@ int skinny_qmm_w4g64_noalloc_errors(void* dst, void* stream);
  * A pool holds n_pages pages; a page holds `page` consecutive positions of one sequence, element
  * [page id][kv head][slot][dim] (dense inside a page; pages k_page_stride / v_page_stride elements
  * apart, a multiple of D; 16-byte aligned).  Sequence b's position j is in slot j % page of page
- * table[b * table_stride + j / page] (int32, width entries per sequence; page * width < 2^31).
+ * table[b * table_stride + j / page] (int32, width entries per sequence; page * width <= 2^31 - 4096).
  * kv_type 0: bf16 pages; 1: e4m3 pages with one f32 scale per kv head (value = stored * scale).
  * D is 64, 128 or 256.
  *

@@ -574,7 +574,7 @@ static int paged_seqs(skinny::PagedSeqs& s, const int32_t* table, long long tabl
                       int page, const int32_t* lengths, const int32_t* counts, int B, int T) {
   if (!table || !lengths) return SKINNY_ERR_INVALID_ARG;
   if (B < 1 || B > skinny::kPagedMaxBatch || T < 1 || static_cast<long long>(B) * T > INT32_MAX) return SKINNY_ERR_SHAPE;
-  if (page < 1 || n_pages < 1 || width < 1 || static_cast<long long>(width) * page > INT32_MAX) return SKINNY_ERR_SHAPE;
+  if (page < 1 || n_pages < 1 || width < 1 || static_cast<long long>(width) * page > skinny::kPagedMaxPositions) return SKINNY_ERR_SHAPE;
   if (table_stride < width && B > 1) return SKINNY_ERR_INVALID_ARG;
   if (!aligned4(table) || !aligned4(lengths) || !aligned4(counts)) return SKINNY_ERR_ALIGNMENT;
   s = skinny::PagedSeqs{lengths, counts, table, table_stride, width, page, n_pages, B, T, nullptr};

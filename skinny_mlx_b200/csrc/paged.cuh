@@ -20,6 +20,7 @@ namespace skinny {
 
 constexpr int kPagedMaxTokens = 16;    // new tokens per sequence of one attention call
 constexpr int kPagedMaxBatch = 8192;   // sequences per call
+constexpr int kPagedMaxPositions = INT32_MAX - 4095;  // of a row of the table: the tile behind the last is still an int
 constexpr int kPagedMaxGroup = 1024;   // query heads per kv head
 
 struct PagedSeqs {

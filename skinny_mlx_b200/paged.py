@@ -31,6 +31,7 @@ _KV_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
 HEAD_DIMS = (64, 128, 256)
 MAX_TOKENS = 16     # new tokens per sequence of one attention call
 MAX_BATCH = 8192
+MAX_POSITIONS = 2**31 - 4096  # of one sequence
 _Strides = ctypes.c_longlong * 3
 
 
@@ -88,8 +89,8 @@ def _seqs(block_table: torch.Tensor, lengths: torch.Tensor, counts, b: int, t: i
         raise ValueError(f"block_table must be int32 [{b}, width] with dense rows on the pages' device")
     if block_table.shape[1] < 1 or (b > 1 and block_table.stride(0) < block_table.shape[1]):
         raise ValueError("block_table needs at least one entry per sequence and rows that do not overlap")
-    if block_table.shape[1] * page > 2**31 - 1:
-        raise ValueError("a sequence's pages must hold fewer than 2^31 positions")
+    if block_table.shape[1] * page > MAX_POSITIONS:
+        raise ValueError(f"a sequence's pages must hold at most {MAX_POSITIONS} positions")
     for name, x in (("lengths", lengths), ("counts", counts)):
         if x is None and name == "counts":
             continue
@@ -282,4 +283,4 @@ def device_errors(device: torch.device | None = None, clear: bool = False) -> in
     return word.value
 
 
-__all__ = ["append", "attention", "device_errors", "PagePool", "PageTable", "HEAD_DIMS", "MAX_BATCH", "MAX_TOKENS"]
+__all__ = ["append", "attention", "device_errors", "PagePool", "PageTable", "HEAD_DIMS", "MAX_BATCH", "MAX_POSITIONS", "MAX_TOKENS"]

@@ -84,6 +84,13 @@ def test_attention_entry_refuses(kw, status):
     assert _attn_status(**kw) == status
 
 
+@pytest.mark.parametrize("status", [_append_status, _attn_status])
+def test_positions_up_to_the_last_tile_are_32_bit(status):
+    """A table whose last tile of keys would end beyond 2^31 is refused."""
+    for width, page in (((1 << 27) - 1, 16), ((1 << 31) - 4095, 1), ((1 << 25) - 63, 64)):
+        assert status(width=width, ts=width, page=page, kps=1 << 20, vps=1 << 20) == -2
+
+
 def test_workspace_of_unsupported_shapes_is_zero():
     from skinny_mlx_b200 import _lib
 
