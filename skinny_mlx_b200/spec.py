@@ -572,17 +572,21 @@ def speculative(model, prompt: list[int], max_tokens: int, drafter, k: int, stat
 
 
 def speculative_tree(model, prompt: list[int], max_tokens: int, drafter, k: int, stats: dict | None = None,
-                     cache=None) -> list[int]:
+                     cache=None, logprobs: list | None = None, top_n: int = 0) -> list[int]:
     """Greedy-exact speculative decoding with a draft TREE verified in one forward (the wider
     drafts the reference proposes to fill the flat-verify budget, docs/flatspec-design.md:64-69):
     each step the drafter proposes tree nodes (draft_tree(k) -> node tokens, parents), the model
     verifies [last token] + nodes with tree attention and a branch-aware GDN recurrence, the
     device walks the tree along the model's own predictions, and the cache keeps the accepted
-    path.  `model` is a HybridModel (module path) or its FusedStep / GraphedStep."""
+    path.  `model` is a HybridModel (module path) or its FusedStep / GraphedStep.  `logprobs` and top_n as for
+    greedy."""
     cache = _fresh_cache(model, cache)
     rb = HybridRollback()
     h, logits = model(torch.tensor(prompt, device=model.device), cache)
     out = [int(torch.argmax(logits[-1].float()))]
+    scored = []
+    if logprobs is not None:
+        scored.append(_logprobs_any(logits[-1:], torch.tensor(out, device=model.device), top_n))
     drafter.begin(prompt, h, out[0])
     steps = accepted = 0
     while len(out) < max_tokens:
@@ -591,6 +595,9 @@ def speculative_tree(model, prompt: list[int], max_tokens: int, drafter, k: int,
         rb.record(cache)
         h, logits = model(x.long(), cache, tree=parent)
         n, new, path = _accept_tree_any(logits, x, parent)
+        if logprobs is not None:
+            rows = logits[torch.tensor(path, device=model.device)]
+            scored.append(_logprobs_any(rows, torch.tensor(new, device=model.device), top_n))
         rb.rollback_tree(cache, fed=x.numel(), path=path)
         drafter.update(h[path[0]:path[0] + 1] if n == 0 else h[torch.tensor(path, device=h.device)], new)
         out += new
@@ -598,6 +605,8 @@ def speculative_tree(model, prompt: list[int], max_tokens: int, drafter, k: int,
         accepted += n
     if stats is not None:
         stats.update(steps=steps, tokens_per_step=len(out) / max(steps, 1), accepted=accepted)
+    if logprobs is not None:
+        logprobs += _read_logprobs(scored)[:max_tokens]
     return out[:max_tokens]
 
 

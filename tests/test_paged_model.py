@@ -11,7 +11,8 @@ from oracle.checks import argmax_violations, rel_err
 from skinny_mlx_b200.dense import DenseModel, small_dense
 from skinny_mlx_b200.model import SMALL, HybridModel, PagedAttnCache
 from skinny_mlx_b200.paged import PagePool, PageTable
-from skinny_mlx_b200.spec import HybridRollback, ScriptedDrafter, greedy, speculative
+from skinny_mlx_b200.spec import (HybridRollback, ScriptedDrafter, ScriptedTreeDrafter, greedy, speculative,
+                                  speculative_tree)
 
 PROMPT = [int(x) for x in np.random.default_rng(5).integers(0, SMALL.vocab, 24)]
 F8 = torch.float8_e4m3fn
@@ -108,6 +109,25 @@ def test_cpu_loops_report_log_probabilities(cpu_model):
         assert abs(r.logprob - lp[i]) < 0.2 and abs(r.entropy - ent[i]) < 0.2
         assert r.top[0][0] == ref[i] and math.isclose(r.top[0][1], r.logprob)
         assert [t[1] for t in r.top] == sorted((t[1] for t in r.top), reverse=True)
+
+
+def _tree_logprobs(model, make_cache, dev):
+    """speculative_tree's report against greedy's, for the same tokens.  A verify's logits are within 1.5e-2 of
+    the largest logit of a single token's (the verify path's bar), so log probabilities x - lse within twice
+    that; the entropy's gradient is -p (ln p + H), of size 2 H at most."""
+    lps, lps2, stats = [], [], {}
+    ref = greedy(model, PROMPT, 9, cache=make_cache(), logprobs=lps, top_n=3)
+    drafter = ScriptedTreeDrafter(ref, 0.6, SMALL.vocab, dev, seed=2)
+    assert speculative_tree(model, PROMPT, 9, drafter, 3, stats, cache=make_cache(), logprobs=lps2, top_n=3) == ref
+    assert stats["accepted"] > 0 and len(lps) == len(lps2) == 9
+    tol = 2 * 1.5e-2 * float(model(torch.tensor(PROMPT + ref[:-1], device=dev), make_cache())[1].float().abs().max())
+    for a, b, t in zip(lps, lps2, ref):
+        assert abs(a.logprob - b.logprob) <= tol and abs(a.entropy - b.entropy) <= tol * a.entropy and len(b.top) == 3
+        assert b.top[0] == (t, b.logprob)
+
+
+def test_cpu_tree_loop_reports_log_probabilities(cpu_model):
+    _tree_logprobs(cpu_model, cpu_model.make_cache, "cpu")
 
 
 # ---------------------------------------------------------------------------------------------
@@ -260,6 +280,13 @@ def test_loops_report_log_probabilities(gpu_model, dev, fused):
         drafter.update(None, [0] * (n + 1))
     assert len(rows) >= 9 and [int(np.argmax(r)) for r in rows[:9]] == got
     _check(lps, np.stack(rows[:9]), got)
+
+
+@pytest.mark.gpu
+def test_tree_loop_reports_log_probabilities(gpu_model, dev):
+    from skinny_mlx_b200.fused import FusedStep, GraphedStep
+
+    _tree_logprobs(GraphedStep(FusedStep(gpu_model)), gpu_model.make_cache, dev)
 
 
 def _check(lps, rows, tokens):
