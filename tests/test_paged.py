@@ -412,6 +412,48 @@ def test_calls_from_two_threads(cuda_lib, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [3, 40, 300])
+def test_a_batch_of_idle_slots(cuda_lib, dev, B):
+    c = Case(dev, [17] * B, counts=[0] * B, T=2)
+    o, lse = c.attend()
+    assert (o == 0).all() and (lse == -math.inf).all()
+    check_append(c, inv_freq(dev, 32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,kv", [(1, torch.bfloat16), (16, F8)])
+def test_attention_of_a_thousand_heads_per_kv_head(cuda_lib, dev, T, kv):
+    c = Case(dev, [100, 3], T=T, Hq=1024, Hkv=1, D=64, kv=kv)
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(window=2**31 - 1), dict(window=300), dict(scale=-0.3), dict(scale=0.0)])
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+def test_attention_extreme_arguments(cuda_lib, dev, kv, kw):
+    c = Case(dev, [250, 0, 77], T=3, kv=kv)
+    check_attention(c.attend(**kw), c.oracle(**kw), c.D)
+
+
+@pytest.mark.gpu
+def test_inputs_of_other_orders(cuda_lib, dev):
+    """Queries, keys and values laid out head by head, a table that is a slice of a wider one, one sequence
+    whose table is an expanded row."""
+    c = Case(dev, [60, 9, 33], T=4, Hq=6, Hkv=2, D=128)
+    swap = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)
+    c.q, c.k, c.v = swap(c.q), swap(c.k), swap(c.v)
+    wide = torch.full((3, c.width + 5), -7, dtype=torch.int32, device=dev)
+    wide[:, 2:2 + c.width] = c.table
+    c.table = wide[:, 2:2 + c.width]
+    check_append(c, inv_freq(dev, 64))
+    check_attention(c.attend(), c.oracle(), c.D)
+    c = Case(dev, [60], T=4)
+    c.table = c.table[0].expand(1, -1)
+    check_append(c, None, with_q=False)
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
 def test_attention_sharp_and_large_scores(cuda_lib, dev):
     """Scores far apart (one key takes everything, late or early) and large ones of both signs."""
     c = Case(dev, [200, 333], T=2, Hq=8, Hkv=2, std=6.0, seed=2)
