@@ -50,6 +50,7 @@
 
 #include "mma_bf16.cuh"
 #include "paged.cuh"
+#include "paged_attn.cuh"
 #include "ptx.cuh"
 
 namespace skinny {
@@ -57,53 +58,6 @@ namespace skinny {
 constexpr int kPtThreads = 128;
 constexpr int kPtWarps = kPtThreads / 32;
 constexpr int kPtLead = 4;             // (0 to 8 tried: verify 31.6 us at 0, 26.2 at 4 and 6, 26.7 at 8; the others hardly move)
-constexpr float kPtMost = 256.f;          // how far p may exceed 1 before the maximum is renewed
-constexpr float kPtNothing = -3.402823466e38f;  // the maximum of a row that has seen no key
-
-struct PagedAttnPlan {
-  int tile_log;    // keys of one tile, one block per warp (a power of two)
-  int lead;        // what beginning an item costs, in tiles: counted on the line, so that the pieces balance
-  int shift;       // log2 of the page size, or -1
-  int box;         // positions of one copy: the largest power of two, up to a block, that divides the page size
-  int nchunk;      // row chunks of 8 NB rows, one per warp (1, 2 or 4); the other warps split keys
-  int groups;      // row groups of nchunk chunks per kv head
-  int join_warps;  // warps per row of the join (a power of two up to 8)
-  int rows;        // rows of one group: 8 NB nchunk
-  int ctas;        // CTAs of the split launch
-  long long* pre;  // [B + 1] where each sequence begins on the line
-  float* ml;       // [2 ctas][rows][2] maximum (log2) and sum of a piece
-  float* o;        // [2 ctas][rows][D]
-  uint32_t rep_inv; // ceil(2^32 / rep), 0 for rep = 1: r / rep of rows r < 2^16
-
-  __device__ __forceinline__ int token(int r) const { return rep_inv ? __umulhi(static_cast<uint32_t>(r), rep_inv) : r; }
-};
-
-// The positions some token of the sequence sees, and the tiles they make.
-struct PagedSpan {
-  int len, cnt, beg, end;
-  int first, tiles;  // the tiles start at a multiple of 32: no box straddles two blocks
-  int units;         // tiles and lead of one item on the line
-};
-
-__device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, const PagedAttnPlan& plan, int b,
-                                                bool* ok = nullptr) {
-  PagedSpan s;
-  const bool good = p.seq.get(b, s.len, s.cnt);
-  if (ok) *ok = good;
-  s.end = s.len + s.cnt;
-  s.beg = p.window > 0 && s.len >= p.window ? s.len - p.window + 1 : 0;
-  s.first = s.beg & ~31;
-  s.tiles = s.cnt > 0 ? ((s.end - s.first - 1) >> plan.tile_log) + 1 : 0;
-  s.units = s.tiles ? s.tiles + plan.lead : 0;
-  return s;
-}
-
-__device__ __forceinline__ float pt_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ uint32_t pt_transpose(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -139,39 +93,6 @@ __device__ __forceinline__ void pt_cvt_e4m3(uint32_t& lo, uint32_t& hi, uint32_t
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
       : "=r"(lo), "=r"(hi)
       : "r"(x));
-}
-
-// a / b of non-negative numbers, in 32 bits where they fit.
-__device__ __forceinline__ long long pt_div(long long a, long long b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
-}
-
-// The line's pieces: `total` units over the CTAs, the first `rest` pieces one unit longer.
-struct PtLine {
-  long long total, each, rest;
-  __device__ __forceinline__ PtLine(long long n, int ctas) : total(n), each(0), rest(0) {
-    const long long parts = min(n, static_cast<long long>(ctas));
-    if (parts > 0) {
-      each = pt_div(n, parts);
-      rest = n - each * parts;
-    }
-  }
-  __device__ __forceinline__ long long start(int i) const { return i * each + min(static_cast<long long>(i), rest); }
-  __device__ __forceinline__ int owner(long long u) const {
-    const long long longer = rest * (each + 1);
-    return static_cast<int>(u < longer ? pt_div(u, each + 1) : rest + pt_div(u - longer, each));
-  }
-};
-
-template <bool F16>
-__device__ __forceinline__ uint32_t pt_pack(float lo, float hi) {
-  if (F16) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Sizes of one instance.
@@ -222,7 +143,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   __shared__ long long scan[kPtWarps];
   __shared__ long long found[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cq = lane & 3;
-  const int rep = p.Hq / p.Hkv, items = p.Hkv * plan.groups, B = p.seq.B;
+  const int rep = p.Hq / p.Hkv, items = p.Hkv * plan.groups;
   const uint32_t bar0 = smem_u32(&bars[warp][0][0]);
   pdl_launch_dependents();
   if (lane < kStages * 2) mbar_init(bar0 + 8 * lane, 1);
@@ -230,83 +151,8 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   fence_mbar_init();
   __syncthreads();
 
-  // ---- this CTA's piece of the line: [u, u_end), beginning `off` units into sequence b
-  int b;
-  long long u, u_end, off;
-  if (B <= 32) {  // one sequence per lane, every warp by itself
-    bool ok = true;
-    const long long mine =
-        lane < B ? static_cast<long long>(paged_span(p, plan, lane, &ok).units) * items : 0;
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    const long long total = __shfl_sync(0xFFFFFFFFu, incl, 31);
-    if (blockIdx.x == 0 && warp == 0) {
-      if (lane < B) plan.pre[lane] = incl - mine;  // the join's copy of the line
-      if (lane == 0) plan.pre[B] = total;
-      if (!ok) atomicOr(p.seq.err, kErrBitBadInput);
-    }
-    if (blockIdx.x >= total) return;
-    const PtLine line(total, plan.ctas);
-    u = line.start(blockIdx.x);
-    u_end = line.start(blockIdx.x + 1);
-    b = __ffs(__ballot_sync(0xFFFFFFFFu, u < incl)) - 1;
-    off = u - __shfl_sync(0xFFFFFFFFu, incl - mine, b);
-  } else {  // thread i sums its run of sequences
-    const int run = (B + kPtThreads - 1) / kPtThreads, b_lo = min(B, tid * run), b_hi = min(B, b_lo + run);
-    long long mine = 0;
-    bool all_ok = true;
-    for (int i = b_lo; i < b_hi; ++i) {
-      bool ok;
-      mine += static_cast<long long>(paged_span(p, plan, i, &ok).units) * items;
-      all_ok &= ok;
-    }
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-      if (lane >= o) incl += x;
-    }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    long long total = 0, excl = incl - mine;
-#pragma unroll
-    for (int w = 0; w < kPtWarps; ++w) {
-      if (w < warp) excl += scan[w];
-      total += scan[w];
-    }
-    if (blockIdx.x == 0) {
-      long long at = excl;
-      for (int i = b_lo; i < b_hi; ++i) {
-        plan.pre[i] = at;
-        at += static_cast<long long>(paged_span(p, plan, i).units) * items;
-      }
-      if (tid == 0) plan.pre[B] = total;
-      if (!all_ok) atomicOr(p.seq.err, kErrBitBadInput);
-    }
-    if (blockIdx.x >= total) return;
-    const PtLine line(total, plan.ctas);
-    u = line.start(blockIdx.x);
-    u_end = line.start(blockIdx.x + 1);
-    if (excl <= u && u < excl + mine) {
-      long long at = excl;
-      for (int i = b_lo; i < b_hi; ++i) {
-        const long long n = static_cast<long long>(paged_span(p, plan, i).units) * items;
-        if (u < at + n) {
-          found[0] = i;
-          found[1] = u - at;
-          break;
-        }
-        at += n;
-      }
-    }
-    __syncthreads();
-    b = static_cast<int>(found[0]);
-    off = found[1];
-  }
+  PtWalk walk;
+  if (!pt_begin<kPtThreads>(p, plan, items, scan, found, walk)) return;
 
   const int chunk = warp % plan.nchunk, slot = warp / plan.nchunk, slots = kPtWarps / plan.nchunk;
   const uint32_t kpr = static_cast<uint32_t>(p.kps / D), vpr = static_cast<uint32_t>(p.vps / D);
@@ -328,22 +174,10 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   uint32_t pending = 0, parity = 0;    // per barrier (bit 2 stage + what): copies in flight, the phase they complete
   bool bad = false;
 
-  for (int seg = 0; u < u_end;) {
-    const PagedSpan sp = paged_span(p, plan, b);
-    if (sp.tiles == 0) {
-      ++b;
-      continue;
-    }
-    const int item = static_cast<int>(pt_div(off, sp.units)), at = static_cast<int>(off - static_cast<long long>(item) * sp.units);
-    const int take = static_cast<int>(min(static_cast<long long>(sp.units - at), u_end - u));
-    const int t0 = max(at - plan.lead, 0), t1 = max(at + take - plan.lead, 0), cur = b;
-    u += take;
-    off += take;
-    if (off == static_cast<long long>(sp.units) * items) {
-      ++b;
-      off = 0;
-    }
-    if (t1 <= t0) continue;  // only an item's lead
+  PtPart part;
+  for (int seg = 0; walk.next(p, plan, items, part);) {
+    const PagedSpan sp = part.sp;
+    const int item = part.item, cur = part.seq, t0 = part.t0, t1 = part.t1;
     const int kvh = item / plan.groups, rbase = (item % plan.groups) * plan.rows;
     const int k0 = sp.first + (t0 << plan.tile_log), k1 = min(sp.end, sp.first + (t1 << plan.tile_log));
     const int r0 = rbase + chunk * 8 * NB;  // this warp's first row
@@ -989,16 +823,51 @@ __global__ void __launch_bounds__(32 * kPtJoinWarps)
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
+cudaError_t pt_encode(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> cached{nullptr};
+  Encode encode = cached.load(std::memory_order_acquire);
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return e;
+    if (!fn || found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    encode = reinterpret_cast<Encode>(fn);
+    cached.store(encode, std::memory_order_release);
+  }
+  const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, steps,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// A pool as [line of 128 bytes][row of D elements][element], to be read in boxes of `lines` lines x `box` rows.
+cudaError_t pt_map(CUtensorMap* map, const void* pool, long long page_stride, const PagedAttnParams& p, int es, int line,
+                   int box, int lines) {
+  const cuuint32_t elems = static_cast<cuuint32_t>(line / es);
+  const cuuint64_t dims[3] = {elems, pt_rows(page_stride, p), static_cast<cuuint64_t>(p.D) / elems};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.D) * es, static_cast<cuuint64_t>(line)};
+  const cuuint32_t boxes[3] = {elems, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(lines)};
+  return pt_encode(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool, dims, strides,
+                   boxes, line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 namespace {
 
 struct PtChoice {
   int nb, nchunk, groups, rows, tile_log, ctas_per_sm;
+  bool tc;  // the tensor-memory kernel
 };
 
 template <int D, int NB, bool F8>
 PtChoice pt_sizes() {
   using S = PtShape<D, NB, F8>;
-  return {NB, 1, 1, 8 * NB, S::kKeys == 32 ? 7 : 6, S::kCtas};
+  return {NB, 1, 1, 8 * NB, S::kKeys == 32 ? 7 : 6, S::kCtas, false};
 }
 
 // As many 8-row blocks per warp as there are, up to what the registers hold; then one chunk of rows
@@ -1016,44 +885,22 @@ PtChoice pt_choose(int T, int Hq, int Hkv) {
   return c;
 }
 
-PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8) {
+// More than 32 rows of bf16 pages go to the tensor-memory kernel, where its copies can be whole rows of 8 keys
+// (`eights`): 64 rows of 16 K contexts 60 us against 96, 128 rows 47 against 104; up to 32 rows the warps' matrix
+// instructions do as well and begin sooner (8 sequences of 4 K: 25 us against 27), and lines of single keys would take
+// it longer (32 rows, pages of 7: 315 us against 117).
+PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8, bool eights) {
+  const int rows = T * (Hq / Hkv);
+  if (!f8 && D <= 128 && eights && rows > 32) {
+    const int chunks = (rows + 31) / 32, nchunk = chunks > 2 ? 4 : 2;
+    return {4, nchunk, (chunks + nchunk - 1) / nchunk, 32 * nchunk, 7, 1, true};
+  }
   if (D == 64) return f8 ? pt_choose<64, true>(T, Hq, Hkv) : pt_choose<64, false>(T, Hq, Hkv);
   if (D == 128) return f8 ? pt_choose<128, true>(T, Hq, Hkv) : pt_choose<128, false>(T, Hq, Hkv);
   return f8 ? pt_choose<256, true>(T, Hq, Hkv) : pt_choose<256, false>(T, Hq, Hkv);
 }
 
 size_t pt_round(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
-
-// A pool as [line of 128 bytes][row of D elements][element], to be read in boxes of `lines` lines x `box` rows.
-// The pages of a pool that interleaves others are further apart: the rows between are never asked for.
-cudaError_t pt_map(CUtensorMap* map, const void* pool, long long page_stride, const PagedAttnParams& p, int es, int line,
-                   int box, int lines) {
-  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static std::atomic<Encode> cached{nullptr};
-  Encode encode = cached.load(std::memory_order_acquire);
-  if (!encode) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
-    if (e != cudaSuccess) return e;
-    if (!fn || found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
-    encode = reinterpret_cast<Encode>(fn);
-    cached.store(encode, std::memory_order_release);
-  }
-  const cuuint64_t rows = static_cast<cuuint64_t>(p.seq.n_pages - 1) * (page_stride / p.D) +
-                          static_cast<cuuint64_t>(p.Hkv) * p.seq.page;
-  const cuuint32_t elems = static_cast<cuuint32_t>(line / es);
-  const cuuint64_t dims[3] = {elems, rows, static_cast<cuuint64_t>(p.D) / elems};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.D) * es, static_cast<cuuint64_t>(line)};
-  const cuuint32_t boxes[3] = {elems, static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(lines)}, steps[3] = {1, 1, 1};
-  const CUresult r = encode(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                            const_cast<void*>(pool), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
 
 template <int D, int NB, bool F8>
 cudaError_t pt_split(const PagedAttnParams& p, const PagedAttnPlan& plan, int dev, cudaLaunchConfig_t cfg) {
@@ -1079,12 +926,14 @@ cudaError_t pt_split(const PagedAttnParams& p, const PagedAttnPlan& plan, int de
 }
 
 template <int D>
-cudaError_t pt_launch(const PagedAttnParams& p, const PagedAttnPlan& plan, int nb, bool f8, int dev, cudaLaunchConfig_t cfg) {
+cudaError_t pt_launch(const PagedAttnParams& p, const PagedAttnPlan& plan, int nb, bool tc, bool f8, int dev,
+                      cudaLaunchConfig_t cfg) {
   cudaError_t e = cudaErrorInvalidValue;
   if (nb == 1) e = f8 ? pt_split<D, 1, true>(p, plan, dev, cfg) : pt_split<D, 1, false>(p, plan, dev, cfg);
   if constexpr (D <= 128) {
     if (nb == 2) e = f8 ? pt_split<D, 2, true>(p, plan, dev, cfg) : pt_split<D, 2, false>(p, plan, dev, cfg);
-    if (nb == 4) e = f8 ? pt_split<D, 4, true>(p, plan, dev, cfg) : pt_split<D, 4, false>(p, plan, dev, cfg);
+    if (tc) e = paged_attn_tc_split(p, plan, dev, cfg);
+    else if (nb == 4) e = f8 ? pt_split<D, 4, true>(p, plan, dev, cfg) : pt_split<D, 4, false>(p, plan, dev, cfg);
   } else {
     if (nb == 2 && f8) e = pt_split<D, 2, true>(p, plan, dev, cfg);
   }
@@ -1100,8 +949,8 @@ cudaError_t pt_launch(const PagedAttnParams& p, const PagedAttnPlan& plan, int n
 
 size_t paged_attn_ws_bytes(int B, int T, int Hq, int Hkv, int D, int n_sm) {
   size_t most = 0;
-  for (int f8 = 0; f8 < 2; ++f8) {
-    const PtChoice c = pt_choose(T, Hq, Hkv, D, f8);
+  for (int i = 0; i < 3; ++i) {
+    const PtChoice c = pt_choose(T, Hq, Hkv, D, i == 2, i == 1);
     const size_t pieces = 2 * static_cast<size_t>(std::max(n_sm, 1)) * c.ctas_per_sm;
     most = std::max(most, pt_round(8 * (static_cast<size_t>(B) + 1)) + pt_round(pieces * c.rows * 8) + pieces * c.rows * D * 4);
   }
@@ -1113,7 +962,8 @@ cudaError_t paged_attn_launch(const PagedAttnParams& p, bool f8, void* ws, int n
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64 || n_sm < 1) return cudaErrorInvalidDevice;
-  const PtChoice c = pt_choose(p.seq.T, p.Hq, p.Hkv, p.D, f8);
+  const bool eights = p.seq.page % 8 == 0 && p.kps / p.D % 8 == 0 && p.vps / p.D % 8 == 0;
+  const PtChoice c = pt_choose(p.seq.T, p.Hq, p.Hkv, p.D, f8, eights);
   PagedAttnPlan plan;
   plan.tile_log = c.tile_log;
   plan.lead = kPtLead;
@@ -1146,9 +996,9 @@ cudaError_t paged_attn_launch(const PagedAttnParams& p, bool f8, void* ws, int n
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (p.D == 64) return pt_launch<64>(p, plan, c.nb, f8, dev, cfg);
-  if (p.D == 128) return pt_launch<128>(p, plan, c.nb, f8, dev, cfg);
-  return pt_launch<256>(p, plan, c.nb, f8, dev, cfg);
+  if (p.D == 64) return pt_launch<64>(p, plan, c.nb, c.tc, f8, dev, cfg);
+  if (p.D == 128) return pt_launch<128>(p, plan, c.nb, c.tc, f8, dev, cfg);
+  return pt_launch<256>(p, plan, c.nb, c.tc, f8, dev, cfg);
 }
 
 }  // namespace skinny

@@ -505,6 +505,85 @@ def test_infinite_values_that_are_seen(cuda_lib, dev):
     assert torch.equal(o.isinf(), hit) and not o.isnan().any()
 
 
+MANY = [(12, 4, 11, 16), (40, 8, 16, 8), (8, 1, 13, 40), (16, 1, 8, 128), (20, 1, 16, 64)]  # 33, 80, 104, 128, 320 rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv,T,page", MANY)
+def test_attention_of_many_rows(cuda_lib, dev, Hq, Hkv, T, page, D):
+    """More than 32 rows per kv head: lengths around a tile's end, idle slots, windows, pools with gaps between
+    pages of which the odd one allows no copies of whole eights, sharp scores."""
+    lengths = [0, 5, 127, 128, 500, 1029, 3, 0]
+    counts = [T, 1, T, 2, 0, T, T - 1, 0]
+    for kw in (dict(), dict(gap=8), dict(gap=3)):
+        c = Case(dev, lengths, counts, T=T, Hq=Hq, Hkv=Hkv, page=page, D=D, seed=Hq + T, **kw)
+        check_attention(c.attend(), c.oracle(), D)
+    c.q = c.q * 6
+    check_attention(c.attend(window=100, scale=-0.2), c.oracle(window=100, scale=-0.2), D)
+    check_attention(c.attend(scale=0.0), c.oracle(scale=0.0), D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,T,page,n", [(12, 4, 11, 16, 9001), (8, 1, 13, 40, 4000), (20, 1, 16, 64, 1500)])
+def test_many_rows_of_long_and_many_sequences(cuda_lib, dev, Hq, Hkv, T, page, n):
+    c = Case(dev, [n, 2], T=T, Hq=Hq, Hkv=Hkv, page=page, seed=3)
+    check_attention(c.attend(), c.oracle(), c.D)
+    lengths = [(53 * i) % 300 for i in range(250)]
+    c = Case(dev, lengths, [T if i % 8 == 5 else i % 3 == 1 for i in range(250)], T=T, Hq=Hq, Hkv=Hkv, page=page, D=64, seed=4)
+    check_attention(c.attend(), c.oracle(), c.D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("Hq,Hkv,T,page", MANY)
+def test_many_rows_and_what_they_do_not_see(cuda_lib, dev, Hq, Hkv, T, page, window):
+    from skinny_mlx_b200 import paged
+
+    lengths = [45, 300, 7]
+    c = Case(dev, lengths, T=T, Hq=Hq, Hkv=Hkv, page=page, seed=T)
+    want = c.attend(window=window)
+    seen = torch.zeros(c.n_pages, page, dtype=torch.bool)
+    for b, n in enumerate(lengths):
+        for j in range(max(0, n + 1 - window) if window else 0, n + T):
+            seen[int(c.table[b, j // page]), j % page] = True
+    for x in (math.nan, math.inf, -math.inf):
+        for pool in (c.kp, c.vp):
+            pool.transpose(1, 2)[(~seen).to(dev)] = x
+        assert all(torch.equal(a, b) for a, b in zip(c.attend(window=window), want))
+    t = T // 2  # a token's own value: the tokens before it do not change
+    for b, n in enumerate(lengths):
+        c.vp[int(c.table[b, (n + t) // page]), :, (n + t) % page] = -math.inf
+    got = c.attend(window=window)
+    # (two roundings of the result, 2^-7 of it, and of the probabilities, 2^-7 sum p |v|)
+    assert all(torch.allclose(a[:, :t].float(), b[:, :t].float(), rtol=2.0 ** -7, atol=2.0 ** -7) for a, b in zip(got, want))
+    assert (got[0][:, t:] == -math.inf).all()
+    # pages of nobody are skipped and reported
+    c.table[1, 1] = c.n_pages
+    c.table[2, :] = -1
+    want = c.oracle(window=window)
+    got = c.attend(window=window)
+    lse = want[1]
+    assert torch.equal(got[1].cpu() > -math.inf, lse > -math.inf) and (got[0][2] == 0).all()
+    assert paged.device_errors(dev, clear=True) == 1 << 9
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,T,page", MANY)
+def test_infinite_values_that_many_rows_see(cuda_lib, dev, Hq, Hkv, T, page):
+    """In a tile that every row sees whole, in either half of it."""
+    c = Case(dev, [1000], T=T, Hq=Hq, Hkv=Hkv, page=page, seed=4)
+    for j, d, x in ((3, 5, math.inf), (100, 77, -math.inf), (200, 0, math.inf), (700, 127, math.nan)):
+        c.vp[int(c.table[0, j // page]), Hkv - 1, j % page, d] = x
+    o = c.attend()[0].float()
+    mine = o[:, :, Hq - Hq // Hkv:]
+    assert (mine[..., 5] == math.inf).all() and (mine[..., 77] == -math.inf).all() and (mine[..., 0] == math.inf).all()
+    assert mine[..., 127].isnan().all()
+    o = o.clone()
+    o[:, :, Hq - Hq // Hkv:, [5, 77, 0, 127]] = 0
+    assert o.isfinite().all()
+
+
 @pytest.mark.gpu
 def test_shared_pages_and_one_page_twice(cuda_lib, dev):
     """Sequences that share a prefix's pages, and a table that names a page twice."""
