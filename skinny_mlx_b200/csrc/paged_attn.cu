@@ -5,6 +5,9 @@
 // over the positions j <= lengths[b] + t of sequence b's pages (and j > lengths[b] + t - window).
 // A row that sees nothing (an idle slot, t >= counts[b], every page bad) is zero, its lse -inf.
 //
+// This file: the split launch for up to 32 rows per kv head, for 8-bit pages and for head dims of 256 (and for any other,
+// where pages are not eights of positions), and the join.  paged_attn_tc.cu: the split launch for more rows.
+//
 // One pass over the cache with a running maximum and sum, split over the cache's length and joined
 // (online softmax).  Bound by the bytes of the keys and values: each is read once from memory, by
 // the warp that multiplies it:
@@ -886,9 +889,10 @@ PtChoice pt_choose(int T, int Hq, int Hkv) {
 }
 
 // More than 32 rows of bf16 pages go to the tensor-memory kernel, where its copies can be whole rows of 8 keys
-// (`eights`): 64 rows of 16 K contexts 60 us against 96, 128 rows 47 against 104; up to 32 rows the warps' matrix
-// instructions do as well and begin sooner (8 sequences of 4 K: 25 us against 27), and lines of single keys would take
-// it longer (32 rows, pages of 7: 315 us against 117).
+// (`eights`): 128 rows of 16 K contexts 49 us against 104, 64 rows of 4 K contexts 28 against 42, 40 rows 27 against
+// 39, of one context of 2 K 16 against 18.  Up to 32 rows the warps' matrix instructions do as well and begin sooner
+// (8 sequences of 4 K: 25 us against 27), and copies of single keys would take it longer (32 rows, pages of 7:
+// 315 us against 117).
 PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8, bool eights) {
   const int rows = T * (Hq / Hkv);
   if (!f8 && D <= 128 && eights && rows > 32) {

@@ -9,12 +9,13 @@
 // lanes, each of which exponentiates half of a tile's keys and multiplies zeros for the others: every warp has
 // the same work, and the halves' O are joined at the item's end.  The matrix unit then repeats itself, which
 // costs nothing: a tile of 128 keys takes it some 1600 clocks, the memory 2700 (64 KB at 1/148 of the copy
-// bandwidth).
+// bandwidth).  Measured: two sequences of 100 K and 64 rows 78 us (80 % of the copy bandwidth), four of 16 K
+// and 128 rows 49 us (exponentials and the row maximum, some 2000 clocks a tile in one warp per scheduler; a
+// CTA's beginning and end, some 10 us, weigh on shorter ones: eight of 4 K and 64 rows 28 us).
 //
-// Seven warps: four of softmax, one that issues the matrix instructions, one that copies keys, one values.  S(n + 1) is computed
-// while the softmax works on S(n); P(n) takes the place of S(n), O += P V follows.  The maximum of a row is
-// renewed only when a score exceeds it by more than 8 (in powers of two), and only then O is read back and
-// rescaled.  Roundings as in paged_attn.cu: p to bf16, all else f32.
+// Seven warps: four of softmax, one that issues the matrix instructions, one that copies keys, one values.
+// S(n + 2) follows O += P(n) V(n), while the softmax works on S(n + 1).  The maximum of a row is renewed only when a
+// score exceeds it by more than 8 (in powers of two), and only then O is read back and rescaled.  Roundings as in paged_attn.cu: p to bf16, all else f32.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -37,21 +38,21 @@ constexpr int kTcORow = kTcHalf + 4;
 template <int D>
 struct TcShape {
   static constexpr int kSlot = kTcKeys * D * 2;             // keys or values of a tile
-  // Slots of the ring.  More for keys, which are freed and asked for ahead of the softmax: their latency is on the
-  // way to the next scores.
-  static constexpr int kKSlots = D == 128 ? 3 : 6, kVSlots = D == 128 ? 2 : 4;
+  // Slots of the ring.  Keys are multiplied two tiles ahead and their slots freed; values stay until their P is there
+  // (3 and 2: 84 us for two sequences of 100 K and 64 rows, 2 and 3: 79).
+  static constexpr int kKSlots = D == 128 ? 2 : 5, kVSlots = D == 128 ? 3 : 5;
   static constexpr int kLines = D / 64;                     // lines of 128 bytes of a row: [key / 8][line][key % 8][128 B]
   static constexpr int kEight = 1024 * kLines;              // bytes of 8 keys
   static constexpr int kSmem = 1024 + kTcRingBytes + 128 * kTcORow * 4;
-  // columns of tensor memory: S (two tiles), O, q
-  static constexpr uint32_t kS = 0, kO = 256, kQ = 384, kCols = 512;
+  // columns of tensor memory: S (two tiles), O, q, P
+  static constexpr uint32_t kS = 0, kO = 256, kQ = 384, kP = 448, kCols = 512;
 };
 
 struct TcShared {
   uint64_t full[10], empty[10];  // per slot of the ring: a tile is there, has been used
   uint64_t info[kTcInfo];    // a tile's `have` is written
   uint64_t s_full[2];        // S(n) is there
-  uint64_t p_full[2];        // P(n) is there, O may be added to
+  uint64_t p_full;           // P(n) is there, O may be added to
   uint64_t pv_done;          // O has P(n) V(n)
   uint64_t q_full;           // a part's q is there
   uint64_t drain;
@@ -111,17 +112,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int rep = p.Hq / p.Hkv, items = p.Hkv * plan.groups;
   const uint32_t ring = smem_u32(smem);
   float* const so = reinterpret_cast<float*>(smem + kTcRingBytes);
-  pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < S::kKSlots + S::kVSlots; ++i) {
       mbar_init(smem_u32(&sh.full[i]), 1);
       mbar_init(smem_u32(&sh.empty[i]), 1);
     }
     for (int i = 0; i < kTcInfo; ++i) mbar_init(smem_u32(&sh.info[i]), 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sh.s_full[i]), 1);
-      mbar_init(smem_u32(&sh.p_full[i]), 128);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sh.s_full[i]), 1);
+    mbar_init(smem_u32(&sh.p_full), 128);
     mbar_init(smem_u32(&sh.pv_done), 1);
     mbar_init(smem_u32(&sh.q_full), 128);
     mbar_init(smem_u32(&sh.drain), 1);
@@ -129,16 +127,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     sh.poison = -1;
     fence_mbar_init();
   }
+  if (warp >= 5) prefetch_tmap(warp == 5 ? &kmap : &vmap);
+  pdl_wait_prior_grid();
   if (warp == 4) {
     tmem_alloc(smem_u32(&sh.tmem), S::kCols);
     tmem_relinquish();
   }
-  if (warp >= 5) prefetch_tmap(warp == 5 ? &kmap : &vmap);
   PtWalk walk;
   const bool some = pt_begin<kTcThreads>(p, plan, items, sh.scan, sh.found, walk);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Only now: a kernel further down the stream may want tensor memory too, before it waits for this one.
+  pdl_launch_dependents();
   const uint32_t tmem = sh.tmem;
   if (!some) {
     if (warp == 4) tmem_dealloc(tmem, S::kCols);
@@ -255,20 +256,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (nt > 1) ok = ok && scores(tile + 1);
       for (int n = 0; ok && n < nt; ++n) {
         const int g = tile + n, slot = v_slot(g);
-        ok = wait(sh.p_full[g & 1], g >> 1) && wait(sh.full[slot], v_turn(g));
+        ok = wait(sh.p_full, g) && wait(sh.full[slot], v_turn(g));
         if (!ok) break;
         tc_fence_after();
         if (lane == 0) {
 #pragma unroll
           for (int k = 0; k < kTcKeys / 16; ++k)
-            umma_f16_ts(tmem + S::kO, tmem + S::kS + (g & 1) * kTcKeys + k * 8,
+            umma_f16_ts(tmem + S::kO, tmem + S::kP + k * 8,
                         tc_desc(ring + slot * S::kSlot + k * 2 * S::kEight, S::kEight), kIdescO, n > 0 || k > 0);
           umma_commit(smem_u32(&sh.empty[slot]));
           umma_commit(smem_u32(&sh.pv_done));
         }
         __syncwarp();
-        // S(n + 2) takes the place of P(n)
-        if (n + 2 < nt) ok = wait(sh.pv_done, g) && scores(g + 2);
+        if (n + 2 < nt) ok = scores(g + 2);  // (every thread has read S(n): it brought P(n))
       }
       tile += nt;
       ++seg;
@@ -287,6 +287,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // scale of 0 makes it 0
     const float sc = p.scale == 0.f ? 1.f : fabsf(p.scale) * 1.4426950408889634f;
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+    if (kSlots > 1) {  // the other half's keys: zeros that stay
+      uint32_t y[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) y[e] = 0u;
+      tmem_st_x32(lanes + S::kP + (1 - slot) * 32, y);
+    }
     int tile = 0;
     for (int seg = 0; walk.next(p, plan, items, part); ++seg) {
       const PagedSpan sp = part.sp;
@@ -320,15 +326,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool ok = true;
       for (int n = 0; n < nt; ++n) {
         const int g = tile + n, j0 = k0 + kTcKeys * n;
-        const uint32_t sp_col = lanes + S::kS + (g & 1) * kTcKeys;
         ok = wait(sh.s_full[g & 1], g >> 1) && wait(sh.info[g % kTcInfo], g / kTcInfo);
         if (!ok) break;
         tc_fence_after();
         float s[kCols];
-        tc_load<kCols>(sp_col + slot * kCols, s);
-        tc_wait_ld();
+        tc_load<kCols>(lanes + S::kS + (g & 1) * kTcKeys + slot * kCols, s);
         const uint4 have = *reinterpret_cast<const uint4*>(sh.have[g % kTcInfo]);
         const bool whole = (have.x & have.y & have.z & have.w) == 0xFFFFFFFFu, edge = is_edge(j0);
+        // Values of keys that do not exist multiply zeros; so do infinities and NaN where some row must not have them
+        // (0 * inf): among values that not every row sees, and with two lane groups anywhere, each of which has
+        // zeros for the other's keys.  The rows that do see them get them after the loop.
+        if (kSlots > 1 || !whole || (p.seq.T > 1 && edge)) {
+          const int vslot = v_slot(g);
+          ok = wait(sh.full[vslot], v_turn(g));
+          if (!ok) break;
+          const bool gone = !(sh.have[g % kTcInfo][warp] >> lane & 1u);
+          // this thread's key, 16 bytes at a time, no two lanes of eight in one bank
+          const uint32_t key = ring + vslot * S::kSlot + (tid >> 3) * S::kEight + (tid & 7) * 128;
+          const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+          __nv_bfloat162 nan[4] = {zero, zero, zero, zero};  // 0 x: NaN and stays so
+#pragma unroll
+          for (int c = 0; c < 8 * S::kLines; ++c) {
+            uint32_t x[4];
+            tc_lds4(x, key + (c >> 3) * 1024 + ((c + lane) & 7) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), zero, nan[e]);
+          }
+          const __nv_bfloat162 any = __hadd2(__hadd2(nan[0], nan[1]), __hadd2(nan[2], nan[3]));
+          const bool odd = !gone && (__hisnan(any.x) || __hisnan(any.y));
+          if (gone || odd) {
+#pragma unroll 1
+            for (int c = 0; c < 8 * S::kLines; ++c) {
+              const uint32_t a = key + (c >> 3) * 1024 + ((c + lane) & 7) * 16;
+              uint32_t x[4];
+              tc_lds4(x, a);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] &= gone ? 0u : ~__vcmpgeu2(x[e] & 0x7FFF7FFFu, 0x7F807F80u);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            }
+            fence_proxy_async_smem();
+          }
+          if (odd) sh.poison = seg;
+        }
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) asm volatile("" : "+f"(s[i]));  // (nothing of it is used before the wait)
         if (!whole || edge) {
 #pragma unroll
           for (int i = 0; i < kCols; ++i) {
@@ -379,52 +421,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           f2_unpack(sum[1], c, d);
           l += (a + b) + (c + d);
         }
-        // P over S; zeros where the keys are other groups'
-#pragma unroll
-        for (int q = 0; q < kSlots; ++q)
-#pragma unroll
-          for (int c = 0; c < kCols / 2; c += 16) {
-            uint32_t y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = q == slot ? pk[c + e] : 0u;
-            tmem_st_x16(sp_col + q * (kCols / 2) + c, y);
-          }
-        // Values of keys that do not exist multiply zeros; so do infinities and NaN where some row must not have them
-        // (0 * inf): among values that not every row sees, and with two lane groups anywhere, each of which has
-        // zeros for the other's keys.  The rows that do see them get them after the loop.
-        if (kSlots > 1 || !whole || (p.seq.T > 1 && edge)) {
-          const int vslot = v_slot(g);
-          ok = wait(sh.full[vslot], v_turn(g));
+        if (n > 0) {  // P(n - 1) has been used
+          ok = wait(sh.pv_done, g - 1);
           if (!ok) break;
-          const bool gone = !(sh.have[g % kTcInfo][warp] >> lane & 1u);
-          // this thread's key, 16 bytes at a time, no two lanes of eight in one bank
-          const uint32_t key = ring + vslot * S::kSlot + (tid >> 3) * S::kEight + (tid & 7) * 128;
-          uint32_t most = 0;
+          tc_fence_after();
+        }
 #pragma unroll
-          for (int c = 0; c < 8 * S::kLines; ++c) {
-            uint32_t x[4];
-            tc_lds4(x, key + (c >> 3) * 1024 + ((c + lane) & 7) * 16);
+        for (int c = 0; c < kCols / 2; c += 32) {
+          uint32_t y[32];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) most = __vmaxu2(most, x[e] & 0x7FFF7FFFu);
-          }
-          const bool odd = !gone && __vcmpgeu2(most, 0x7F807F80u) != 0;
-          if (gone || odd) {
-#pragma unroll 1
-            for (int c = 0; c < 8 * S::kLines; ++c) {
-              const uint32_t a = key + (c >> 3) * 1024 + ((c + lane) & 7) * 16;
-              uint32_t x[4];
-              tc_lds4(x, a);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] &= gone ? 0u : ~__vcmpgeu2(x[e] & 0x7FFF7FFFu, 0x7F807F80u);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-            }
-            fence_proxy_async_smem();
-          }
-          if (odd) sh.poison = seg;
+          for (int e = 0; e < 32; ++e) y[e] = pk[c + e];
+          tmem_st_x32(lanes + S::kP + slot * (kCols / 2) + c, y);
         }
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&sh.p_full[g & 1]));
+        mbar_arrive(smem_u32(&sh.p_full));
       }
       tile += nt;
 
@@ -552,8 +563,7 @@ static cudaError_t tc_split(const PagedAttnParams& p, const PagedAttnPlan& plan,
   if (e == cudaSuccess) e = tc_map(&vmap, p.vp, p.vps, p, plan.box);
   if (e != cudaSuccess) return e;
   cfg.blockDim = dim3(kTcThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.numAttrs = 0;  // (not a dependent launch, as in paged_attn.cu)
+  cfg.dynamicSmemBytes = S::kSmem;  // (one CTA per SM: a dependent launch places them evenly)
   return cudaLaunchKernelEx(&cfg, kernel, p, plan, kmap, vmap);
 }
 
