@@ -5,8 +5,8 @@
 // over the positions j <= lengths[b] + t of sequence b's pages (and j > lengths[b] + t - window).
 // A row that sees nothing (an idle slot, t >= counts[b], every page bad) is zero, its lse -inf.
 //
-// This file: the split launch for up to 32 rows per kv head, for 8-bit pages and for head dims of 256 (and for any other,
-// where pages are not eights of positions), and the join.  paged_attn_tc.cu: the split launch for more rows.
+// This file: the split launch for few rows per kv head, for 8-bit pages and for pages that are not eights of positions,
+// and the join.  paged_attn_tc.cu: the split launch for more rows.
 //
 // One pass over the cache with a running maximum and sum, split over the cache's length and joined
 // (online softmax).  Bound by the bytes of the keys and values: each is read once from memory, by
@@ -888,16 +888,17 @@ PtChoice pt_choose(int T, int Hq, int Hkv) {
   return c;
 }
 
-// More than 32 rows of bf16 pages go to the tensor-memory kernel, where its copies can be whole rows of 8 keys
-// (`eights`): 128 rows of 16 K contexts 49 us against 104, 64 rows of 4 K contexts 28 against 42, 40 rows 27 against
-// 39, of one context of 2 K 16 against 18.  Up to 32 rows the warps' matrix instructions do as well and begin sooner
-// (8 sequences of 4 K: 25 us against 27), and copies of single keys would take it longer (32 rows, pages of 7:
-// 315 us against 117).
+// More than 32 rows of bf16 pages (16 of heads of 256) go to the tensor-memory kernel, where its copies can be whole
+// rows of 8 keys (`eights`): 128 rows of 16 K contexts 49 us against 104, 64 rows of 4 K contexts 28 against 42, 40
+// rows 27 against 39, 64 rows of one context of 2 K 16 against 18; heads of 256, 4 K contexts: 64 rows 46 against 97,
+// 20 rows 39 against 56.  With fewer the warps' matrix instructions do as well and begin sooner (32 rows of 8
+// sequences of 4 K: 25 us against 27; heads of 256, 10 rows: 36 against 38), and copies of single keys would take the
+// other longer (32 rows, pages of 7: 315 us against 117).
 PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8, bool eights) {
   const int rows = T * (Hq / Hkv);
-  if (!f8 && D <= 128 && eights && rows > 32) {
+  if (!f8 && eights && rows > (D == 256 ? 16 : 32)) {
     const int chunks = (rows + 31) / 32, nchunk = chunks > 2 ? 4 : 2;
-    return {4, nchunk, (chunks + nchunk - 1) / nchunk, 32 * nchunk, 7, 1, true};
+    return {4, nchunk, (chunks + nchunk - 1) / nchunk, 32 * nchunk, D == 256 ? 6 : 7, 1, true};
   }
   if (D == 64) return f8 ? pt_choose<64, true>(T, Hq, Hkv) : pt_choose<64, false>(T, Hq, Hkv);
   if (D == 128) return f8 ? pt_choose<128, true>(T, Hq, Hkv) : pt_choose<128, false>(T, Hq, Hkv);
@@ -933,11 +934,13 @@ template <int D>
 cudaError_t pt_launch(const PagedAttnParams& p, const PagedAttnPlan& plan, int nb, bool tc, bool f8, int dev,
                       cudaLaunchConfig_t cfg) {
   cudaError_t e = cudaErrorInvalidValue;
-  if (nb == 1) e = f8 ? pt_split<D, 1, true>(p, plan, dev, cfg) : pt_split<D, 1, false>(p, plan, dev, cfg);
-  if constexpr (D <= 128) {
+  if (tc) {
+    e = paged_attn_tc_split(p, plan, dev, cfg);
+  } else if (nb == 1) {
+    e = f8 ? pt_split<D, 1, true>(p, plan, dev, cfg) : pt_split<D, 1, false>(p, plan, dev, cfg);
+  } else if constexpr (D <= 128) {
     if (nb == 2) e = f8 ? pt_split<D, 2, true>(p, plan, dev, cfg) : pt_split<D, 2, false>(p, plan, dev, cfg);
-    if (tc) e = paged_attn_tc_split(p, plan, dev, cfg);
-    else if (nb == 4) e = f8 ? pt_split<D, 4, true>(p, plan, dev, cfg) : pt_split<D, 4, false>(p, plan, dev, cfg);
+    if (nb == 4) e = f8 ? pt_split<D, 4, true>(p, plan, dev, cfg) : pt_split<D, 4, false>(p, plan, dev, cfg);
   } else {
     if (nb == 2 && f8) e = pt_split<D, 2, true>(p, plan, dev, cfg);
   }
@@ -974,7 +977,7 @@ cudaError_t paged_attn_launch(const PagedAttnParams& p, bool f8, void* ws, int n
   plan.shift = -1;
   for (int i = 0; i < 31; ++i)
     if (p.seq.page == 1 << i) plan.shift = i;
-  plan.box = 1 << (c.tile_log - 2);  // a block's keys
+  plan.box = c.tc ? 32 : 1 << (c.tile_log - 2);  // a block's keys
   while (p.seq.page % plan.box) plan.box /= 2;
   const uint32_t rep = static_cast<uint32_t>(p.Hq / p.Hkv);
   plan.rep_inv = rep == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + rep - 1) / rep);

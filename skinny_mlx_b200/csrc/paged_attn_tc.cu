@@ -1,8 +1,8 @@
 // Paged attention of many query rows (tokens x heads of a kv head) on the tensor-memory matrix units: the split
-// launch for bf16 pages whose item has more than 16 rows; the line, its pieces and the join are those of
-// paged_attn.cu.
+// launch for bf16 pages whose items have many rows (the rule is pt_choose's); the line, its pieces and the join are
+// those of paged_attn.cu.
 //
-// A tile is 128 keys.  S = q K^T has the query rows in the 128 lanes of tensor memory and the keys in its
+// A tile is 128 keys (64 of heads of 256).  S = q K^T has the query rows in the 128 lanes of tensor memory and the keys in its
 // columns, so a thread owns a row: its maximum, its sum and its part of O need no exchange.  q and P are
 // operands in tensor memory, K (rows of D) and V (D in the other direction) come by TMA into a ring in shared
 // memory and are read there as they lie.  With 64 rows per item the rows are repeated in both halves of the
@@ -29,7 +29,6 @@
 namespace skinny {
 
 constexpr int kTcThreads = 224;
-constexpr int kTcKeys = 128;         // of one tile
 constexpr int kTcRingBytes = 163840;
 constexpr int kTcInfo = 8;           // tiles whose flags are kept: keys are asked for at most 8 tiles ahead of the softmax
 constexpr int kTcHalf = 64;          // dims of O that pass through shared memory at a time
@@ -37,15 +36,21 @@ constexpr int kTcORow = kTcHalf + 4;
 
 template <int D>
 struct TcShape {
-  static constexpr int kSlot = kTcKeys * D * 2;             // keys or values of a tile
+  static constexpr int kKeys = D == 256 ? 64 : 128;         // of one tile
+  static constexpr int kWords = kKeys / 32;
+  static constexpr int kSlot = kKeys * D * 2;               // keys or values of a tile
   // Slots of the ring.  Keys are multiplied two tiles ahead and their slots freed; values stay until their P is there
   // (3 and 2: 84 us for two sequences of 100 K and 64 rows, 2 and 3: 79).
-  static constexpr int kKSlots = D == 128 ? 2 : 5, kVSlots = D == 128 ? 3 : 5;
+  static constexpr int kKSlots = D == 64 ? 5 : 2, kVSlots = D == 64 ? 5 : 3;
   static constexpr int kLines = D / 64;                     // lines of 128 bytes of a row: [key / 8][line][key % 8][128 B]
   static constexpr int kEight = 1024 * kLines;              // bytes of 8 keys
   static constexpr int kSmem = 1024 + kTcRingBytes + 128 * kTcORow * 4;
-  // columns of tensor memory: S (two tiles), O, q, P
-  static constexpr uint32_t kS = 0, kO = 256, kQ = 384, kP = 448, kCols = 512;
+  // Columns of tensor memory: S (two tiles), O, q, P.  Heads of 256 fill it without P, which takes the place of its
+  // S then (and S(n + 2) waits for P(n) V(n)).
+  static constexpr bool kOver = D == 256;
+  static constexpr uint32_t kS = 0, kO = 2 * kKeys, kQ = 384, kP = 448, kCols = 512;
+  static_assert(kO + D <= kQ && kQ + D / 2 <= (kOver ? 512 : kP), "tensor memory");
+  __device__ static __forceinline__ uint32_t p_col(int g) { return kOver ? kS + (g & 1) * kKeys : kP; }
 };
 
 struct TcShared {
@@ -57,7 +62,7 @@ struct TcShared {
   uint64_t q_full;           // a part's q is there
   uint64_t drain;
   alignas(16) uint32_t have[kTcInfo][4]; // the keys of a tile that exist
-  uint32_t rows[2][kTcKeys]; // the copying warps' own: where a tile's keys (values) lie
+  uint32_t rows[2][128];     // the copying warps' own: where a tile's keys (values) lie
   float ml[128][2];          // per lane: maximum and sum
   float weight[4][128];      // per lane group and row: what its O counts
   float inv[128];
@@ -82,11 +87,18 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t eight) {
   return d;
 }
 
-__device__ __forceinline__ void tc_softmax_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void tc_softmax_barrier() {  // of the softmax warps, each whole behind it
+  __syncwarp();
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  __syncwarp();
+}
 
 __device__ __forceinline__ void tc_lds4(uint32_t (&x)[4], uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
 }
+
+__device__ __forceinline__ void tc_store(uint32_t taddr, const uint32_t (&v)[16]) { tmem_st_x16(taddr, v); }
+__device__ __forceinline__ void tc_store(uint32_t taddr, const uint32_t (&v)[32]) { tmem_st_x32(taddr, v); }
 
 template <int N>
 __device__ __forceinline__ void tc_load(uint32_t taddr, float (&s)[N]) {
@@ -104,7 +116,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     paged_attn_tc_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ PagedAttnPlan plan,
                          const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using S = TcShape<D>;
-  constexpr int kCols = 32 * NC, kSlots = 4 / NC;  // keys of a tile that a lane group has, lane groups with the same rows
+  // lane groups with the same rows, and the keys of a tile that each has
+  constexpr int kKeys = S::kKeys, kSlots = 4 / NC, kCols = kKeys / kSlots;
   extern __shared__ __align__(1024) uint8_t tc_raw[];
   uint8_t* const smem = tc_raw + ((1024 - (smem_u32(tc_raw) & 1023)) & 1023);
   __shared__ TcShared sh;
@@ -148,7 +161,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // bounded waits of a whole warp: the same answer in every lane
   const auto wait = [&](const uint64_t& bar, uint32_t parity) {
     const bool ok = mbar_wait(smem_u32(&bar), parity & 1u, p.seq.err, kErrBitWaitFull, &sh.gave_up);
-    return __all_sync(0xFFFFFFFFu, ok) != 0;
+    const bool all = __all_sync(0xFFFFFFFFu, ok) != 0;
+    __syncwarp();
+    return all;
   };
   // tile g's keys (values): their slot, and how often it has been used before
   const auto k_slot = [](int g) { return g % S::kKSlots; };
@@ -172,11 +187,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int nt = part.t1 - part.t0;
       const int k0 = sp.first + (part.t0 << plan.tile_log), k1 = min(sp.end, sp.first + (part.t1 << plan.tile_log));
       const int32_t* const table = p.seq.table + part.seq * p.seq.table_stride;
-      int pid[4], in_page[4];
+      int pid[S::kWords], in_page[S::kWords];
       const auto look = [&](int n) {  // tile n's pages, one key per lane and 32 keys
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int j = k0 + kTcKeys * n + 32 * w + lane;
+        for (int w = 0; w < S::kWords; ++w) {
+          const int j = k0 + kKeys * n + 32 * w + lane;
           pid[w] = -2;
           in_page[w] = 0;
           if (n < nt && j >= sp.beg && j < k1) {
@@ -188,11 +203,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       look(0);
       for (int n = 0; n < nt; ++n, ++tile) {
-        uint32_t ex[4];
+        uint32_t ex[4] = {0u, 0u, 0u, 0u};
         __syncwarp();  // (the rows of the tile before have been read)
         int there = 0;  // boxes with a key that exists
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < S::kWords; ++w) {
           const bool here = pid[w] >= 0 && pid[w] < p.seq.n_pages;
           bad |= !here && pid[w] != -2;
           sh.rows[kv][32 * w + lane] = static_cast<uint32_t>(pid[w]) * per + head + static_cast<uint32_t>(in_page[w]);
@@ -209,7 +224,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t bar = smem_u32(&sh.full[slot]), dst = ring + slot * S::kSlot;
         if (lane == 0) mbar_arrive_expect_tx(bar, there * plan.box * 2 * D);
         __syncwarp();
-        if (lane < 4 * boxes) {  // one copy per lane
+        if (lane < S::kWords * boxes) {  // one copy per lane
           const int w = lane / boxes, first = (lane & (boxes - 1)) * plan.box;
           const uint32_t here = (w == 0 ? ex[0] : w == 1 ? ex[1] : w == 2 ? ex[2] : ex[3]) & mask << first;
           if (here) {
@@ -229,7 +244,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
   } else if (warp == 4) {
     // ---- matrix instructions, issued by lane 0
-    constexpr uint32_t kIdescS = idesc_bf16_f32(128, kTcKeys);
+    constexpr uint32_t kIdescS = idesc_bf16_f32(128, kKeys);
     constexpr uint32_t kIdescO = idesc_bf16_f32(128, D) | 1u << 16;  // (B's N direction is the contiguous one)
     bool ok = true;
     int tile = 0, seg = 0;
@@ -240,7 +255,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (lane == 0) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_f16_ts(tmem + S::kS + (g & 1) * kTcKeys, tmem + S::kQ + k * 8,
+          umma_f16_ts(tmem + S::kS + (g & 1) * kKeys, tmem + S::kQ + k * 8,
                       tc_desc(ring + slot * S::kSlot + (k / 4) * 1024 + (k % 4) * 32, S::kEight), kIdescS, k > 0);
         umma_commit(smem_u32(&sh.empty[slot]));
         umma_commit(smem_u32(&sh.s_full[g & 1]));
@@ -261,14 +276,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         if (lane == 0) {
 #pragma unroll
-          for (int k = 0; k < kTcKeys / 16; ++k)
-            umma_f16_ts(tmem + S::kO, tmem + S::kP + k * 8,
+          for (int k = 0; k < kKeys / 16; ++k)
+            umma_f16_ts(tmem + S::kO, tmem + S::p_col(g) + k * 8,
                         tc_desc(ring + slot * S::kSlot + k * 2 * S::kEight, S::kEight), kIdescO, n > 0 || k > 0);
           umma_commit(smem_u32(&sh.empty[slot]));
           umma_commit(smem_u32(&sh.pv_done));
         }
         __syncwarp();
-        if (n + 2 < nt) ok = scores(g + 2);  // (every thread has read S(n): it brought P(n))
+        // (every thread has read S(n): it brought P(n))
+        if (n + 2 < nt) ok = (!S::kOver || wait(sh.pv_done, g)) && scores(g + 2);
       }
       tile += nt;
       ++seg;
@@ -287,12 +303,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // scale of 0 makes it 0
     const float sc = p.scale == 0.f ? 1.f : fabsf(p.scale) * 1.4426950408889634f;
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    if (kSlots > 1) {  // the other half's keys: zeros that stay
-      uint32_t y[32];
+    const uint32_t zeros[16] = {};
+    const auto others = [&](int g) {  // zeros for the other half's keys
+      if (kSlots > 1)
 #pragma unroll
-      for (int e = 0; e < 32; ++e) y[e] = 0u;
-      tmem_st_x32(lanes + S::kP + (1 - slot) * 32, y);
-    }
+        for (int c = 0; c < kCols / 2; c += 16) tmem_st_x16(lanes + S::p_col(g) + (1 - slot) * (kCols / 2) + c, zeros);
+    };
+    if (!S::kOver) others(0);  // (they stay)
     int tile = 0;
     for (int seg = 0; walk.next(p, plan, items, part); ++seg) {
       const PagedSpan sp = part.sp;
@@ -312,6 +329,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             x[4 * e + 2] = w.z ^ flip;
             x[4 * e + 3] = w.w ^ flip;
           }
+          __syncwarp();
           tmem_st_x32(lanes + S::kQ + 32 * i, x);
         }
         tc_wait_st();
@@ -320,61 +338,64 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       const int last = sp.len + t, least = p.window > 0 ? last - p.window + 1 : 0;  // the positions this row sees
       const auto is_edge = [&](int j0) {  // a tile that some row sees only part of
-        return j0 + kTcKeys - 1 > sp.len || (p.window > 0 && j0 <= sp.len + sp.cnt - 1 - p.window);
+        return j0 + kKeys - 1 > sp.len || (p.window > 0 && j0 <= sp.len + sp.cnt - 1 - p.window);
       };
       float m = kPtNothing, l = 0.f;
       bool ok = true;
       for (int n = 0; n < nt; ++n) {
-        const int g = tile + n, j0 = k0 + kTcKeys * n;
+        const int g = tile + n, j0 = k0 + kKeys * n;
         ok = wait(sh.s_full[g & 1], g >> 1) && wait(sh.info[g % kTcInfo], g / kTcInfo);
         if (!ok) break;
         tc_fence_after();
         float s[kCols];
-        tc_load<kCols>(lanes + S::kS + (g & 1) * kTcKeys + slot * kCols, s);
+        tc_load<kCols>(lanes + S::kS + (g & 1) * kKeys + slot * kCols, s);
         const uint4 have = *reinterpret_cast<const uint4*>(sh.have[g % kTcInfo]);
-        const bool whole = (have.x & have.y & have.z & have.w) == 0xFFFFFFFFu, edge = is_edge(j0);
+        const bool whole = (have.x & have.y & (S::kWords == 4 ? have.z & have.w : ~0u)) == ~0u, edge = is_edge(j0);
         // Values of keys that do not exist multiply zeros; so do infinities and NaN where some row must not have them
         // (0 * inf): among values that not every row sees, and with two lane groups anywhere, each of which has
         // zeros for the other's keys.  The rows that do see them get them after the loop.
-        if (kSlots > 1 || !whole || (p.seq.T > 1 && edge)) {
-          const int vslot = v_slot(g);
-          ok = wait(sh.full[vslot], v_turn(g));
-          if (!ok) break;
-          const bool gone = !(sh.have[g % kTcInfo][warp] >> lane & 1u);
-          // this thread's key, 16 bytes at a time, no two lanes of eight in one bank
-          const uint32_t key = ring + vslot * S::kSlot + (tid >> 3) * S::kEight + (tid & 7) * 128;
-          const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
-          __nv_bfloat162 nan[4] = {zero, zero, zero, zero};  // 0 x: NaN and stays so
+        const uint32_t key = ring + v_slot(g) * S::kSlot + (tid >> 3) * S::kEight + (tid & 7) * 128;
+        bool gone = false, odd = false;
+        const auto look = [&]() {  // this thread's key, 16 bytes at a time, no two lanes of eight in one bank
+          if (!wait(sh.full[v_slot(g)], v_turn(g))) return false;
+          if (warp < S::kWords) {
+            gone = !(sh.have[g % kTcInfo][warp] >> lane & 1u);
+            const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+            __nv_bfloat162 nan[4] = {zero, zero, zero, zero};  // 0 x: NaN and stays so
 #pragma unroll
-          for (int c = 0; c < 8 * S::kLines; ++c) {
-            uint32_t x[4];
-            tc_lds4(x, key + (c >> 3) * 1024 + ((c + lane) & 7) * 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) nan[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), zero, nan[e]);
-          }
-          const __nv_bfloat162 any = __hadd2(__hadd2(nan[0], nan[1]), __hadd2(nan[2], nan[3]));
-          const bool odd = !gone && (__hisnan(any.x) || __hisnan(any.y));
-          if (gone || odd) {
-#pragma unroll 1
             for (int c = 0; c < 8 * S::kLines; ++c) {
-              const uint32_t a = key + (c >> 3) * 1024 + ((c + lane) & 7) * 16;
               uint32_t x[4];
-              tc_lds4(x, a);
+              tc_lds4(x, key + (c >> 3) * 1024 + ((c + lane) & 7) * 16);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] &= gone ? 0u : ~__vcmpgeu2(x[e] & 0x7FFF7FFFu, 0x7F807F80u);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+              for (int e = 0; e < 4; ++e) nan[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), zero, nan[e]);
             }
-            fence_proxy_async_smem();
+            const __nv_bfloat162 any = __hadd2(__hadd2(nan[0], nan[1]), __hadd2(nan[2], nan[3]));
+            odd = !gone && (__hisnan(any.x) || __hisnan(any.y));
           }
-          if (odd) sh.poison = seg;
-        }
+          return true;
+        };
+        if ((kSlots > 1 || !whole || (p.seq.T > 1 && edge)) && !(ok = look())) break;  // (the scores are on their way)
         tc_wait_ld();
 #pragma unroll
         for (int i = 0; i < kCols; ++i) asm volatile("" : "+f"(s[i]));  // (nothing of it is used before the wait)
+        if (gone || odd) {
+#pragma unroll 1
+          for (int c = 0; c < 8 * S::kLines; ++c) {
+            const uint32_t a = key + (c >> 3) * 1024 + ((c + lane) & 7) * 16;
+            uint32_t x[4];
+            tc_lds4(x, a);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] &= gone ? 0u : ~__vcmpgeu2(x[e] & 0x7FFF7FFFu, 0x7F807F80u);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+          fence_proxy_async_smem();
+          if (odd) sh.poison = seg;
+        }
+        __syncwarp();  // (tensor memory is for whole warps)
         if (!whole || edge) {
 #pragma unroll
           for (int i = 0; i < kCols; ++i) {
-            const uint32_t word = sh.have[g % kTcInfo][slot * NC + i / 32];
+            const uint32_t word = sh.have[g % kTcInfo][slot * (kCols / 32) + i / 32];
             const int j = j0 + slot * kCols + i;
             if (!(word >> (i & 31) & 1u) || j > last || j < least) s[i] = -INFINITY;
           }
@@ -421,17 +442,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           f2_unpack(sum[1], c, d);
           l += (a + b) + (c + d);
         }
-        if (n > 0) {  // P(n - 1) has been used
+        if (n > 0) {  // P(n - 1) has been used (and this warp cannot arrive twice at one turn of p_full)
           ok = wait(sh.pv_done, g - 1);
           if (!ok) break;
           tc_fence_after();
         }
+        if (S::kOver) others(g);
+        constexpr int kStore = kCols / 2 < 32 ? 16 : 32;
 #pragma unroll
-        for (int c = 0; c < kCols / 2; c += 32) {
-          uint32_t y[32];
+        for (int c = 0; c < kCols / 2; c += kStore) {
+          uint32_t y[kStore];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = pk[c + e];
-          tmem_st_x32(lanes + S::kP + slot * (kCols / 2) + c, y);
+          for (int e = 0; e < kStore; ++e) y[e] = pk[c + e];
+          tc_store(lanes + S::p_col(g) + slot * (kCols / 2) + c, y);
         }
         tc_wait_st();
         tc_fence_before();
@@ -482,7 +505,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int32_t* const table = p.seq.table + part.seq * p.seq.table_stride;
 #pragma unroll 1
           for (int n = 0; n < nt; ++n) {
-            const int j0 = k0 + kTcKeys * n;
+            const int j0 = k0 + kKeys * n;
 #pragma unroll 1
             for (int j = j0 + slot * kCols; (kSlots > 1 || is_edge(j0)) && j < min(j0 + (slot + 1) * kCols, k1); ++j) {
               const int pid = table[j / p.seq.page];
@@ -569,7 +592,8 @@ static cudaError_t tc_split(const PagedAttnParams& p, const PagedAttnPlan& plan,
 
 cudaError_t paged_attn_tc_split(const PagedAttnParams& p, const PagedAttnPlan& plan, int dev, const cudaLaunchConfig_t& cfg) {
   if (p.D == 64) return plan.nchunk == 2 ? tc_split<64, 2>(p, plan, dev, cfg) : tc_split<64, 4>(p, plan, dev, cfg);
-  return plan.nchunk == 2 ? tc_split<128, 2>(p, plan, dev, cfg) : tc_split<128, 4>(p, plan, dev, cfg);
+  if (p.D == 128) return plan.nchunk == 2 ? tc_split<128, 2>(p, plan, dev, cfg) : tc_split<128, 4>(p, plan, dev, cfg);
+  return plan.nchunk == 2 ? tc_split<256, 2>(p, plan, dev, cfg) : tc_split<256, 4>(p, plan, dev, cfg);
 }
 
 }  // namespace skinny

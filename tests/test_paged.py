@@ -585,6 +585,28 @@ def test_infinite_values_that_many_rows_see(cuda_lib, dev, Hq, Hkv, T, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,T,page", MANY)
+def test_many_rows_of_wide_heads(cuda_lib, dev, Hq, Hkv, T, page):
+    """Heads of 256: values, windows and scales, a longer sequence, and infinities that are seen or not."""
+    c = Case(dev, [0, 63, 64, 500, 1029, 3], [T, T, 1, 0, T - 1, 2], T=T, Hq=Hq, Hkv=Hkv, page=page, D=256, seed=Hq, gap=8)
+    check_attention(c.attend(), c.oracle(), 256)
+    c.q = c.q * 6
+    check_attention(c.attend(window=100, scale=-0.2), c.oracle(window=100, scale=-0.2), 256)
+    c = Case(dev, [3000], T=T, Hq=Hq, Hkv=Hkv, page=page, D=256, seed=5)
+    want = c.attend()
+    check_attention(want, c.oracle(), 256)
+    c.vp[int(c.table[0, 70 // page]), Hkv - 1, 70 % page, 200] = math.inf  # every row sees it
+    j = 3000 + T // 2                                                      # rows from T / 2 on see it
+    c.vp[int(c.table[0, j // page]), 0, j % page, 31] = -math.inf
+    o = c.attend()[0].float()
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[:, :, Hq - Hq // Hkv:, 200] = True
+    hit[:, T // 2:, :Hq // Hkv, 31] = True
+    assert torch.equal(o.isinf(), hit) and not o.isnan().any()
+    assert torch.allclose(o[~hit], want[0].float()[~hit], rtol=2.0 ** -7, atol=2.0 ** -7)  # (two roundings, as above)
+
+
+@pytest.mark.gpu
 def test_shared_pages_and_one_page_twice(cuda_lib, dev):
     """Sequences that share a prefix's pages, and a table that names a page twice."""
     c = Case(dev, [70, 90, 64], T=1, Hq=4, Hkv=2, page=16, seed=8)
