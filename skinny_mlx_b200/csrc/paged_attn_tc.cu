@@ -2,8 +2,8 @@
 // launch for bf16 pages whose items have many rows (the rule is pt_choose's); the line, its pieces and the join are
 // those of paged_attn.cu.
 //
-// A tile is 128 keys (64 of heads of 256).  S = q K^T has the query rows in the 128 lanes of tensor memory and the keys in its
-// columns, so a thread owns a row: its maximum, its sum and its part of O need no exchange.  q and P are
+// A tile is 128 keys (64 of heads of 256).  S = q K^T has the query rows in the 128 lanes of tensor memory and
+// the keys in its columns, so a thread owns a row: its maximum, its sum and its part of O need no exchange.  q and P are
 // operands in tensor memory, K (rows of D) and V (D in the other direction) come by TMA into a ring in shared
 // memory and are read there as they lie.  With 64 rows per item the rows are repeated in both halves of the
 // lanes, each of which exponentiates half of a tile's keys and multiplies zeros for the others: every warp has
@@ -15,7 +15,8 @@
 //
 // Seven warps: four of softmax, one that issues the matrix instructions, one that copies keys, one values.
 // S(n + 2) follows O += P(n) V(n), while the softmax works on S(n + 1).  The maximum of a row is renewed only when a
-// score exceeds it by more than 8 (in powers of two), and only then O is read back and rescaled.  Roundings as in paged_attn.cu: p to bf16, all else f32.
+// score exceeds it by more than 8 (in powers of two), and only then O is read back and rescaled.
+// Roundings as in paged_attn.cu: p to bf16, all else f32.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
