@@ -585,6 +585,45 @@ def test_infinite_values_that_many_rows_see(cuda_lib, dev, Hq, Hkv, T, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hkv,D", [(4, 128), (2, 128), (2, 256)])
+def test_many_rows_on_two_streams_and_replayed(cuda_lib, dev, Hkv, D):
+    """Two batches at a time, eagerly and from graphs whose lengths change between replays: the bits of calls one
+    after the other."""
+    cases = [Case(dev, [700 + 91 * i, 5, 2000], T=16, Hq=16, Hkv=Hkv, D=D, page=32, seed=i, width=70) for i in range(2)]
+    lengths = [[(c.lengths - 3 * n * (c.lengths > 100)).int() for n in range(4)] for c in cases]
+    want = []
+    for c, ls in zip(cases, lengths):
+        want.append([])
+        for n in ls:
+            c.lengths = n
+            want[-1].append(c.attend())
+    check_attention(want[1][3], cases[1].oracle(), D)
+    streams = [torch.cuda.Stream(dev) for _ in cases]
+    for c, ls in zip(cases, lengths):
+        c.lengths = ls[0].clone()
+    torch.cuda.synchronize()
+    graphs = []
+    for c, s in zip(cases, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = [c.attend() for _ in range(3)]
+        graphs.append((g, out))
+    for n in range(4):
+        eager = []
+        for c, ls, s in zip(cases, lengths, streams):
+            with torch.cuda.stream(s):
+                c.lengths.copy_(ls[n])
+                eager.append([c.attend() for _ in range(3)])
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for got in eager[i] + graphs[i][1]:
+                assert all(torch.equal(x, y) for x, y in zip(got, want[i][n]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("Hq,Hkv,T,page", MANY)
 def test_many_rows_of_wide_heads(cuda_lib, dev, Hq, Hkv, T, page):
     """Heads of 256: values, windows and scales, a longer sequence, and infinities that are seen or not."""
