@@ -30,12 +30,14 @@
 // * P^T as an operand is the transpose of the S^T accumulators, one movmatrix per 8 x 8 block.
 //
 // The maximum a row's exponentials refer to is renewed only when a score exceeds it by more than
-// 8 (in powers of two): p stays below 256, which bf16 and f16 hold at the same relative precision,
-// and the usual block needs one warp vote instead of shuffles and a rescaling of O.
-// Roundings: scores, maxima, sums and O are f32; p is rounded to bf16 (bf16 pages: half a step, as
-// the output's own rounding) or f16 (e4m3 pages: keys and values are exact in f16, and q is scaled
-// per row by a power of two so that it is exact too).  The sum adds the p before that rounding, so
-// the lse does not see it.
+// 8 (in powers of two): p stays below 256, and the usual block needs one warp vote instead of shuffles and
+// a rescaling of O.
+// Roundings: scores, maxima, sums and O are f32; p is rounded to bf16 (half a step, as the output's own
+// rounding), the same relative precision however far a key lies below the row's largest.  The sum adds the p
+// before that rounding, so the lse does not see it.  e4m3 keys and values are exact in bf16 and converted in
+// registers.  (f16 is one instruction nearer, but its smallest number is 2^-24: keys 17 nats below a dominating
+// one, and elements of q far below the row's largest, were lost.  f16 against bf16: 64 sequences up to 4 K 73.5
+// and 73 us, two of 131 K 95.5 and 93, 16 rows of 16 K 35 and 39, heads of 64 54.5 and 64.5, of 256 32.6 and 35.)
 //
 // Work split: the key tiles of all (sequence, kv head, row group) items form one line that is cut
 // into equal pieces, one per CTA (`kCtas` CTAs per SM), so that ragged lengths balance; the
@@ -67,21 +69,13 @@ __device__ __forceinline__ uint32_t pt_transpose(uint32_t x) {
   return y;
 }
 
-template <bool F16>
 __device__ __forceinline__ void pt_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-  if (F16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void pt_lds4(uint32_t (&r)[4], uint32_t a) {
@@ -91,11 +85,18 @@ __device__ __forceinline__ void pt_lds2(uint32_t& x, uint32_t& y, uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(a) : "memory");
 }
 
-// Two pairs of e4m3 to two pairs of f16 (exact; NaN stays NaN).
+// Two pairs of e4m3 to two pairs of bf16 (exact, NaN stays NaN): by way of f16, of which bf16 is the upper half in f32.
+__device__ __forceinline__ uint32_t pt_f16_to_bf16(uint32_t x) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+  return __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+}
 __device__ __forceinline__ void pt_cvt_e4m3(uint32_t& lo, uint32_t& hi, uint32_t x) {
+  uint32_t a, b;
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-      : "=r"(lo), "=r"(hi)
+      : "=r"(a), "=r"(b)
       : "r"(x));
+  lo = pt_f16_to_bf16(a);
+  hi = pt_f16_to_bf16(b);
 }
 
 // Sizes of one instance.
@@ -142,7 +143,6 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
   __shared__ uint64_t bars[kPtWarps][kStages][2];  // per warp and stage: the block (its keys, its values) is there
   __shared__ int gave_up;                          // a wait ran out
   __shared__ float sml[kPtWarps][8 * NB][2];
-  __shared__ float sdown[S::kChunks * 8 * NB];  // e4m3: the power of two each row's q was divided by
   __shared__ long long scan[kPtWarps];
   __shared__ long long found[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cq = lane & 3;
@@ -305,23 +305,13 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
     }
 
     // ---- the query rows to shared memory
-    const float sc0 = p.scale * 1.4426950408889634f * (F8 ? p.k_scale[kvh] : 1.f);
+    const float sc = p.scale * 1.4426950408889634f * (F8 ? p.k_scale[kvh] : 1.f);
     const auto q_store = [&](int e, uint4 w) {
       const int row = e / (D / 8), u8 = e % (D / 8);
       uint8_t* const dst = sq + row * S::kQPad;
-      if (F8) {  // to f16, the row's largest |q| to [1, 2); pairs 0, 2, .. of 16 dims before pairs 1, 3, ..
-        uint32_t x[4] = {w.x, w.y, w.z, w.w}, top = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) top = max(top, max(x[c] & 0x7FFFu, (x[c] >> 16) & 0x7FFFu));
-#pragma unroll
-        for (int o = 1; o < D / 8; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const uint32_t ex = min(max(top >> 7, 1u), 253u);
-        const float up = top >= 0x7F80u ? 1.f : __uint_as_float((254u - ex) << 23);
-        if (u8 == 0) sdown[row] = top >= 0x7F80u ? 1.f : __uint_as_float(ex << 23);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          *reinterpret_cast<uint32_t*>(dst + (u8 >> 1) * 32 + (c & 1) * 16 + (u8 & 1) * 8 + (c >> 1) * 4) =
-              pt_pack<true>(__uint_as_float(x[c] << 16) * up, __uint_as_float(x[c] & 0xFFFF0000u) * up);
+      if (F8) {  // pairs 0, 2, .. of 16 dims before pairs 1, 3, ..
+        *reinterpret_cast<uint2*>(dst + (u8 >> 1) * 32 + (u8 & 1) * 8) = make_uint2(w.x, w.z);
+        *reinterpret_cast<uint2*>(dst + (u8 >> 1) * 32 + 16 + (u8 & 1) * 8) = make_uint2(w.y, w.w);
       } else {
         reinterpret_cast<uint4*>(dst)[u8] = w;
       }
@@ -347,15 +337,6 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
           uint32_t(&x)[4] = qr[S::kQRegs ? nb : 0][S::kQRegs ? i : 0];
           ldsm_x4(qaddr + nb * 8 * S::kQPad + i * 64, x[0], x[1], x[2], x[3]);
         }
-    }
-    float sc[F8 ? NB : 1][2];  // the factor that takes a score to powers of two
-    if (F8) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) sc[F8 ? nb : 0][e] = sc0 * sdown[chunk * 8 * NB + 8 * nb + 2 * cq + e];
-    } else {
-      sc[0][0] = sc[0][1] = sc0;
     }
     // the tokens of this lane's rows, 4 bits each (rows past the last token: any)
     uint32_t tokens = 0;
@@ -445,7 +426,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
               a3 = kw[sub][3];
             }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) pt_mma<F8>(s[nb][sub], a0, a1, a2, a3, bq[nb][0], bq[nb][1]);
+            for (int nb = 0; nb < NB; ++nb) pt_mma(s[nb][sub], a0, a1, a2, a3, bq[nb][0], bq[nb][1]);
           }
         }
       }
@@ -456,7 +437,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
 #pragma unroll
         for (int sub = 0; sub < kSub; ++sub)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nb][sub][e] *= sc[F8 ? nb : 0][e & 1];
+          for (int e = 0; e < 4; ++e) s[nb][sub][e] *= sc;
       if (is_edge(j0) || now != kAll) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -517,8 +498,8 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
           const float(&x)[4] = pr[nb][sub];
           l[nb][0] += x[0] + x[2];
           l[nb][1] += x[1] + x[3];
-          pb[nb][sub][0] = pt_transpose(pt_pack<F8>(x[0], x[1]));
-          pb[nb][sub][1] = pt_transpose(pt_pack<F8>(x[2], x[3]));
+          pb[nb][sub][0] = pt_transpose(pt_pack(x[0], x[1]));
+          pb[nb][sub][1] = pt_transpose(pt_pack(x[2], x[3]));
         }
       if (!S::kJoint && !arrived(stage * 2 + 1)) break;
       if (now != kAll) {  // keys that do not exist multiply zeros
@@ -577,14 +558,14 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
                 pt_cvt_e4m3(a2, a3, __byte_perm(v[2][c], v[3][c], hf ? 0x7362 : 0x5140));
                 const int q = F8 ? 2 * (i * (S::kVBytes / 4) + c) + hf : 0;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) pt_mma<true>(o[nb][q], a0, a1, a2, a3, pb[nb][sub][0], pb[nb][sub][1]);
+                for (int nb = 0; nb < NB; ++nb) pt_mma(o[nb][q], a0, a1, a2, a3, pb[nb][sub][0], pb[nb][sub][1]);
               }
             } else {
               const uint32_t a0 = __byte_perm(v[0][c], v[1][c], 0x5410), a1 = __byte_perm(v[0][c], v[1][c], 0x7632),
                              a2 = __byte_perm(v[2][c], v[3][c], 0x5410), a3 = __byte_perm(v[2][c], v[3][c], 0x7632);
               const int q = F8 ? 0 : 4 * i + c;
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) pt_mma<false>(o[nb][q], a0, a1, a2, a3, pb[nb][sub][0], pb[nb][sub][1]);
+              for (int nb = 0; nb < NB; ++nb) pt_mma(o[nb][q], a0, a1, a2, a3, pb[nb][sub][0], pb[nb][sub][1]);
             }
           }
         }
@@ -705,7 +686,7 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
         }
         if (whole)
           *reinterpret_cast<uint2*>(p.out + row * D + d) =
-              make_uint2(pt_pack<false>(acc.x * iv, acc.y * iv), pt_pack<false>(acc.z * iv, acc.w * iv));
+              make_uint2(pt_pack(acc.x * iv, acc.y * iv), pt_pack(acc.z * iv, acc.w * iv));
         else
           *reinterpret_cast<float4*>(plan.o + (piece * plan.rows + r) * D + d) = acc;
       }

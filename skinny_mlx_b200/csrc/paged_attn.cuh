@@ -5,7 +5,6 @@
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "paged.cuh"
@@ -83,12 +82,7 @@ struct PtLine {
   }
 };
 
-template <bool F16>
 __device__ __forceinline__ uint32_t pt_pack(float lo, float hi) {
-  if (F16) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }

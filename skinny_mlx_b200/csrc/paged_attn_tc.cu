@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           a = pt_exp2(a);
           b = pt_exp2(b);
           sum[i / 2 & 1] = f2_fma(f2_pack(a, b), one, sum[i / 2 & 1]);
-          pk[i / 2] = pt_pack<false>(a, b);
+          pk[i / 2] = pt_pack(a, b);
         }
         {
           float a, b, c, d;
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (entire) {
             const float iv = sh.inv[q];
             *reinterpret_cast<uint2*>(p.out + static_cast<size_t>(sh.row_out[q]) * D + d0 + quad) =
-                make_uint2(pt_pack<false>(acc.x * iv, acc.y * iv), pt_pack<false>(acc.z * iv, acc.w * iv));
+                make_uint2(pt_pack(acc.x * iv, acc.y * iv), pt_pack(acc.z * iv, acc.w * iv));
           } else {
             *reinterpret_cast<float4*>(plan.o + (piece * plan.rows + q) * D + d0 + quad) = acc;
           }

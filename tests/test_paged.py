@@ -761,3 +761,63 @@ def test_python_refusals(cuda_lib, dev):
     assert paged.attention(q=c.q[:0], **z).shape == (0, 2, 4, 128)
     assert paged.append(c.q[:0], c.k[:0], c.v[:0], **z).shape == (0, 2, 4, 128)
     assert paged.device_errors(dev) == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# keys that take nearly all of a row
+# ---------------------------------------------------------------------------------------------
+def _sink(dev, kv, T, lengths, at, nats, **kw):
+    """Sequences in which the key at position at(length), of value 0, lies `nats` above all others for every row
+    (scale 1): dim 0 of the queries is 8 and of the other keys 0, the other dims give scores of some +-0.5."""
+    c = Case(dev, lengths, T=T, kv=kv, std=0.2, **kw)
+    ks = torch.ones(c.Hkv) if c.scales["k_scale"] is None else c.scales["k_scale"].cpu()
+    c.q = c.q.clone()
+    c.q[..., 0] = 8
+    c.kp[..., 0] = 0
+    for b, n in enumerate(lengths):
+        j = at(n)
+        pid = int(c.table[b, j // c.page])
+        for h in range(c.Hkv):
+            c.kp[pid, h, j % c.page] = 0
+            c.kp[pid, h, j % c.page, 0] = (nats / 8 / ks[h]).to(kv).to(dev)
+        c.vp[pid, :, j % c.page] = 0
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("T", [1, 8, 16])
+@pytest.mark.parametrize("nats", [10, 14, 16, 17, 18, 20, 22, 25, 40])
+def test_one_key_takes_nearly_all(cuda_lib, dev, T, nats, kv):
+    """First, in the middle, last: what the other keys add keeps its relative precision however little it is.  (The
+    bounds are check_attention's: each p is off by half a bf16 step, 2^-8 of itself, whatever its size.)"""
+    for at in (lambda n: 0, lambda n: n // 2, lambda n: n - 1):
+        c = _sink(dev, kv, T, [1500, 300, 40], at, nats, Hq=8, Hkv=2, page=16, seed=nats)
+        check_attention(c.attend(scale=1.0), c.oracle(scale=1.0), c.D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 2, 2), (64, 16, 1), (256, 2, 1), (256, 16, 1)])
+def test_one_key_takes_nearly_all_of_other_heads(cuda_lib, dev, D, Hq, Hkv):
+    for T in (1, 4):
+        c = _sink(dev, F8, T, [1500, 300, 40], lambda n: 0, 20, Hq=Hq, Hkv=Hkv, D=D, page=32, seed=D)
+        check_attention(c.attend(scale=1.0), c.oracle(scale=1.0), D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [torch.bfloat16, F8])
+@pytest.mark.parametrize("power", [10, 16, 26, 60, 120])
+def test_query_elements_far_apart(cuda_lib, dev, power, kv):
+    """One element of a query row is 2^power and meets keys that are 0 there: the others keep their precision.
+    The same with an infinity, which gives NaN in its own row alone."""
+    c = Case(dev, [300, 40], T=3, Hq=4, Hkv=2, kv=kv, seed=power)
+    c.q = c.q.clone()
+    c.q[:, :, 1::2, 5] = 2.0 ** power
+    c.kp[..., 5] = 0
+    check_attention(c.attend(), c.oracle(), c.D)
+    want = c.attend()[0]
+    c.q[:, 1, 1, 5] = math.inf
+    got = c.attend()[0]
+    assert got[:, 1, 1].isnan().all()
+    got[:, 1, 1] = want[:, 1, 1]
+    assert torch.equal(got, want)
