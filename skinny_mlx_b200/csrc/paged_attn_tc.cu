@@ -503,12 +503,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         if (sh.poison == seg) {  // the infinities and NaN that were left out, to the rows that see them
+          // (of every tile: where none was left out, its infinity or NaN is in O already and once more changes nothing)
           const int32_t* const table = p.seq.table + part.seq * p.seq.table_stride;
 #pragma unroll 1
           for (int n = 0; n < nt; ++n) {
             const int j0 = k0 + kKeys * n;
 #pragma unroll 1
-            for (int j = j0 + slot * kCols; (kSlots > 1 || is_edge(j0)) && j < min(j0 + (slot + 1) * kCols, k1); ++j) {
+            for (int j = j0 + slot * kCols; j < min(j0 + (slot + 1) * kCols, k1); ++j) {
               const int pid = table[j / p.seq.page];
               if (j < sp.beg || pid < 0 || pid >= p.seq.n_pages) continue;
               const __nv_bfloat16* const src = static_cast<const __nv_bfloat16*>(p.vp) + pid * static_cast<size_t>(p.vps) +

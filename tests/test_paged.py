@@ -821,3 +821,29 @@ def test_query_elements_far_apart(cuda_lib, dev, power, kv):
     assert got[:, 1, 1].isnan().all()
     got[:, 1, 1] = want[:, 1, 1]
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,T,page,D", [(8, 1, 13, 40, 128), (20, 1, 16, 16, 128), (16, 1, 8, 8, 64), (8, 1, 16, 16, 256),
+                                             (12, 4, 11, 16, 128), (8, 2, 3, 16, 128), (4, 2, 1, 16, 64)])
+def test_infinite_values_beside_a_page_that_is_skipped(cuda_lib, dev, Hq, Hkv, T, page, D):
+    """A page id outside the pool in the middle of a context, infinities and NaN in the tile around it: only the
+    page is skipped, every row gets what it sees of the others."""
+    from skinny_mlx_b200 import paged
+
+    paged.device_errors(dev, clear=True)
+    c = Case(dev, [1000, 400], T=T, Hq=Hq, Hkv=Hkv, page=page, D=D, seed=9)
+    c.table[0, 160 // page] = c.n_pages  # keys 160 to 160 + page
+    want = c.oracle()
+    for j, d, x in ((150, 5, math.inf), (155, 33, -math.inf), (210, 9, math.nan), (1000, 40, math.inf)):
+        c.vp[int(c.table[0, j // page]), Hkv - 1, j % page, d] = x
+    got = c.attend()
+    assert paged.device_errors(dev, clear=True) == 1 << 9
+    o = got[0].float()
+    mine = o[0, :, Hq - Hq // Hkv:]
+    assert (mine[..., 5] == math.inf).all() and (mine[..., 33] == -math.inf).all() and mine[..., 9].isnan().all()
+    assert (mine[..., 40] == math.inf).all()
+    got[0][0, :, Hq - Hq // Hkv:, [5, 9, 33, 40]] = 0
+    for x in (want[0], want[2]):
+        x[0, :, Hq - Hq // Hkv:, [5, 9, 33, 40]] = 0
+    check_attention(got, want, D)
