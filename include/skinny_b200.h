@@ -371,7 +371,8 @@ int skinny_qmm_w4g64_noalloc_errors(void* dst, void* stream);
  * [page id][kv head][slot][dim] (dense inside a page; pages k_page_stride / v_page_stride elements
  * apart, a multiple of D; 16-byte aligned).  Sequence b's position j is in slot j % page of page
  * table[b * table_stride + j / page] (int32, width entries per sequence; page * width <= 2^31 - 4096).
- * kv_type 0: bf16 pages; 1: e4m3 pages with one f32 scale per kv head (value = stored * scale).
+ * kv_type 0: bf16 pages, k_scale and v_scale NULL; 1: e4m3 pages with one f32 scale per kv head
+ * (k_scale, v_scale [Hkv]; value = stored * scale).
  * D is 64, 128 or 256.
  *
  * lengths [B] int32 (device): the tokens in the cache BEFORE the step; counts [B] int32 (device, may

@@ -581,9 +581,9 @@ static int paged_seqs(skinny::PagedSeqs& s, const int32_t* table, long long tabl
   return SKINNY_OK;
 }
 
-// Pages of a pool: aligned, dense inside a page, the scales of an 8-bit pool.
+// Pages of a pool: aligned, dense inside a page, with scales if and only if they are of 8 bits.
 static int check_pages(const void* p, long long stride, int kv_type, const float* scale, int Hkv, int page, int D) {
-  if (!p || kv_type < 0 || kv_type > 1 || (kv_type == 1 && !scale)) return SKINNY_ERR_INVALID_ARG;
+  if (!p || kv_type < 0 || kv_type > 1 || (kv_type == 1) != (scale != nullptr)) return SKINNY_ERR_INVALID_ARG;
   if (Hkv < 1 || Hkv > 1024 || (D != 64 && D != 128 && D != 256)) return SKINNY_ERR_SHAPE;
   if (stride < static_cast<long long>(Hkv) * page * D) return SKINNY_ERR_INVALID_ARG;
   if (!aligned16(p) || stride % D || !aligned4(scale)) return SKINNY_ERR_ALIGNMENT;

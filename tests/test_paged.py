@@ -91,6 +91,13 @@ def test_positions_up_to_the_last_tile_are_32_bit(status):
         assert status(width=width, ts=width, page=page, kps=1 << 20, vps=1 << 20) == -2
 
 
+@pytest.mark.parametrize("status", [_append_status, _attn_status])
+@pytest.mark.parametrize("kw", [dict(ksc=F), dict(vsc=F), dict(ksc=F, vsc=F)])
+def test_scales_of_16_bit_pages_are_refused(status, kw):
+    """(The join of split items would apply them, items that one CTA has whole would not.)"""
+    assert status(**kw) == -1
+
+
 def test_workspace_of_unsupported_shapes_is_zero():
     from skinny_mlx_b200 import _lib
 
