@@ -220,6 +220,9 @@ class PagePool:
             raise ValueError("layers, n_pages, n_kv_heads and page must be at least 1")
         if dtype == torch.bfloat16 and (k_scale is not None or v_scale is not None):
             raise ValueError("scales are for float8_e4m3fn pages")
+        for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if x is not None and tuple(x.shape) != (layers, n_kv_heads):
+                raise ValueError(f"{name} must be [{layers}, {n_kv_heads}], got {tuple(x.shape)}")
         self.page, self.n_pages, self.dtype = page, n_pages, dtype
         shape = (layers, n_pages, n_kv_heads, page, head_dim)
         self.k, self.v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))

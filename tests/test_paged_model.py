@@ -49,6 +49,16 @@ def test_pool_and_table_bookkeeping():
             PagePool(**{**dict(layers=2, n_pages=5, n_kv_heads=2, head_dim=64, page=4, device="cpu"), **bad})
 
 
+@pytest.mark.parametrize("shape", [(2,), (3,), (3, 1), (1, 2), (2, 3), (3, 2, 1), (4, 2)])
+def test_pool_scales_of_another_shape_are_refused(shape):
+    """One scale per layer and kv head: anything else would be spread over dims or layers that it was not made for."""
+    for name in ("k_scale", "v_scale"):
+        with pytest.raises(ValueError, match=name):
+            PagePool(3, 5, 2, 64, 4, dtype=F8, device="cpu", **{name: torch.ones(shape)})
+    pool = PagePool(3, 5, 2, 64, 4, dtype=F8, device="cpu", k_scale=torch.full((3, 2), 0.5))
+    assert [s.tolist() for s in pool.k_scale] == [[0.5, 0.5]] * 3 and [s.tolist() for s in pool.v_scale] == [[1.0, 1.0]] * 3
+
+
 def test_caches_refuse_foreign_pools_and_trees(cpu_model):
     with pytest.raises(ValueError, match="pool"):
         cpu_model.make_cache(pool=PagePool(2, 5, 2, 128, 4, device="cpu"))
