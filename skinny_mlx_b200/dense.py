@@ -141,7 +141,8 @@ class DenseModel(nn.Module):
 
     def make_cache(self, max_len: int = 4096, pool=None) -> list[AttnCache]:
         """pool: a paged.PagePool of cfg.layers layers and this rank's kv heads, instead of contiguous buffers
-        (the caches' shared page table, `caches[0].table`, is released by the caller)."""
+        (the caches' shared page table, `caches[0].table`, is released by the caller, who sets their lengths to 0
+        before they are used again)."""
         c = self.cfg
         if pool is not None:
             from .paged import PageTable

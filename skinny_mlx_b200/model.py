@@ -207,7 +207,7 @@ class PagedAttnCache(AttnCache):
         from . import paged
 
         T, L0 = q.shape[0], self.length
-        self.table.reserve(L0 + T)
+        self.table.reserve(L0 + T, L0)
         self.length = L0 + T
         kp, vp = self.pool.k[self.layer], self.pool.v[self.layer]
         ks, vs = self.pool.k_scale[self.layer], self.pool.v_scale[self.layer]
@@ -550,7 +550,7 @@ class HybridModel(nn.Module):
         if cache.table is not None:  # what a paged cache refuses, before any layer's state has changed
             if tree is not None:
                 raise ValueError("a tree verify needs a contiguous cache")
-            cache.table.reserve(cache.offset + ids.shape[0])
+            cache.table.reserve(cache.offset + ids.shape[0], cache.offset)
         x = self.embed_tokens(ids)
         for layer, c in zip(self.layers, cache.layers):
             x = layer(x, c, tree)

@@ -254,9 +254,12 @@ class PageTable:
         self.width = -(-max_len // pool.page)
         self.device = torch.full((1, max(self.width, 1)), -1, dtype=torch.int32, device=pool.k.device)
 
-    def reserve(self, length: int) -> None:
-        """Pages for the first `length` positions (those that are there stay)."""
+    def reserve(self, length: int, cached: int = 0) -> None:
+        """Pages for the first `length` positions (those that are there stay).  Of `cached` of them something is
+        already stored: without their pages, released meanwhile, nothing is reserved."""
         need = -(-length // self.pool.page)
+        if cached > len(self.pages) * self.pool.page:
+            raise ValueError(f"the pages of {cached} cached positions have been released: empty the cache first")
         if need > self.width:
             raise ValueError(f"{length} positions do not fit a cache of {self.width * self.pool.page}")
         n = len(self.pages)

@@ -106,6 +106,35 @@ def test_a_refused_step_changes_no_state(cpu_model):
     assert torch.equal(m(y, c)[1], want)
 
 
+def test_a_step_on_released_pages_is_refused(cpu_model):
+    """Once a table's pages are back in the pool its cached positions are gone: a step that would read them from
+    whatever pages it got next is refused, and goes on when the cache is emptied."""
+    m = cpu_model
+    pool = m.make_pool(20, 7)
+    c = m.make_cache(pool=pool)
+    x = torch.tensor(PROMPT)
+    want = m(x, c)[1]
+    state = [g.state.clone() for g in c.layers if not isinstance(g, PagedAttnCache)]
+    c.table.release()
+    with pytest.raises(ValueError, match="released"):
+        m(torch.tensor([3]), c)
+    assert c.offset == len(PROMPT) and pool.free_pages == 20
+    assert all(torch.equal(g.state, s) for g, s in zip((g for g in c.layers if not isinstance(g, PagedAttnCache)), state))
+    c.reset()
+    assert torch.equal(m(x, c)[1], want)
+    d = DenseModel(small_dense(), seed=3, device="cpu")
+    pool = PagePool(2, 20, 8, 128, 16, device="cpu")
+    caches = d.make_cache(64, pool=pool)
+    want = d(x, caches)
+    caches[0].table.release()
+    with pytest.raises(ValueError, match="released"):
+        d(torch.tensor([3]), caches)
+    for c in caches:
+        assert c.length == len(PROMPT)
+        c.length = 0
+    assert torch.equal(d(x, caches), want)
+
+
 def test_cpu_loops_report_log_probabilities(cpu_model):
     m = cpu_model
     lps, lps2 = [], []
