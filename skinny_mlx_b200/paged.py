@@ -231,6 +231,7 @@ class PagePool:
             one = lambda s: torch.ones(layers, n_kv_heads, device=device) if s is None else s
             self.k_scale, self.v_scale = (list(one(s).to(device, torch.float32).contiguous()) for s in (k_scale, v_scale))
         self._free = list(range(n_pages - 1, -1, -1))
+        self._taken: set[int] = set()
 
     @property
     def free_pages(self) -> int:
@@ -240,9 +241,15 @@ class PagePool:
         """n pages of nobody; raises when there are not as many."""
         if n > len(self._free):
             raise RuntimeError(f"the page pool is exhausted: {n} pages wanted, {len(self._free)} of {self.n_pages} free")
-        return [self._free.pop() for _ in range(n)]
+        pages = [self._free.pop() for _ in range(n)]
+        self._taken.update(pages)
+        return pages
 
     def give(self, pages: list[int]) -> None:
+        """Pages that were taken, back to nobody; a page that nobody has would later be two sequences'."""
+        if len(set(pages)) != len(pages) or not self._taken.issuperset(pages):
+            raise ValueError("only pages that are taken can be given back, each once")
+        self._taken.difference_update(pages)
         self._free.extend(pages)
 
 

@@ -106,6 +106,21 @@ def test_a_refused_step_changes_no_state(cpu_model):
     assert torch.equal(m(y, c)[1], want)
 
 
+def test_a_page_is_given_back_once():
+    pool = PagePool(1, 6, 2, 64, 4, device="cpu")
+    a = pool.take(3)
+    for bad in ([a[0], a[0]], [next(i for i in range(6) if i not in a)], [6], [-1], [a[0], 7]):
+        with pytest.raises(ValueError, match="given back"):
+            pool.give(bad)
+        assert pool.free_pages == 3
+    pool.give(a[:2])
+    with pytest.raises(ValueError, match="given back"):
+        pool.give(a)
+    pool.give(a[2:])
+    assert sorted(pool.take(6)) == list(range(6)) and pool.free_pages == 0
+    pool.give([])
+
+
 def test_a_step_on_released_pages_is_refused(cpu_model):
     """Once a table's pages are back in the pool its cached positions are gone: a step that would read them from
     whatever pages it got next is refused, and goes on when the cache is emptied."""
