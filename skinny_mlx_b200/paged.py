@@ -80,6 +80,8 @@ def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale, v_scale) -> int
 
 
 def _page_stride(x: torch.Tensor) -> int:
+    if x.numel() == 0:
+        raise ValueError("a pool holds at least one page of one kv head and one position")
     return x.stride(0) if x.shape[0] > 1 else x[0].numel()
 
 

@@ -854,3 +854,20 @@ def test_infinite_values_beside_a_page_that_is_skipped(cuda_lib, dev, Hq, Hkv, T
     for x in (want[0], want[2]):
         x[0, :, Hq - Hq // Hkv:, [5, 9, 33, 40]] = 0
     check_attention(got, want, D)
+
+
+@pytest.mark.gpu
+def test_pools_of_nothing_are_refused(cuda_lib, dev):
+    from skinny_mlx_b200 import paged
+
+    c = Case(dev, [5, 9], T=2, Hq=4, Hkv=2)
+    for cut in (lambda x: x[:0], lambda x: x[:, :, :0], lambda x: x[:1, :, :0]):
+        with pytest.raises(ValueError):
+            paged.attention(c.q, cut(c.kp), cut(c.vp), c.table, c.lengths)
+        with pytest.raises(ValueError):
+            paged.append(c.q, c.k, c.v, cut(c.kp), cut(c.vp), c.table, c.lengths)
+    none = [x[:, :0] for x in (c.kp, c.vp)]
+    with pytest.raises(ValueError):
+        paged.attention(c.q, *none, c.table, c.lengths)
+    with pytest.raises(ValueError):
+        paged.append(None, c.k[:, :, :0], c.v[:, :, :0], *none, c.table, c.lengths)
