@@ -147,8 +147,9 @@ class DenseModel(nn.Module):
         if pool is not None:
             from .paged import PageTable
 
-            if pool.k.shape[0] != c.layers or tuple(pool.k.shape[2::2]) != (c.n_kv_heads // self.world, c.head_dim):
-                raise ValueError("the pool has other layers or heads than the model")
+            if pool.k.shape[0] != c.layers or pool.k.device != torch.empty(0, device=self.device).device or tuple(
+                    pool.k.shape[2::2]) != (c.n_kv_heads // self.world, c.head_dim):
+                raise ValueError("the pool has other layers, heads or another device than the model")
             table = PageTable(pool, max_len)
             return [PagedAttnCache(pool, table, i) for i in range(c.layers)]
         shard = type("C", (), {"n_kv_heads": c.n_kv_heads // self.world, "head_dim": c.head_dim})

@@ -71,6 +71,16 @@ def test_caches_refuse_foreign_pools_and_trees(cpu_model):
         cpu_model(torch.tensor([1, 2, 3]), c, tree=[-1, 0, 0])
 
 
+def test_caches_refuse_pools_of_another_device(cpu_model):
+    """When the cache is made, not in a step that has already counted its tokens."""
+    n = cpu_model.make_pool(4).k.shape[0]
+    with pytest.raises(ValueError, match="device"):
+        cpu_model.make_cache(pool=PagePool(n, 5, SMALL.n_kv_heads, SMALL.head_dim, 4, device="meta"))
+    d = DenseModel(small_dense(), seed=3, device="cpu")
+    with pytest.raises(ValueError, match="device"):
+        d.make_cache(64, pool=PagePool(2, 5, 8, 128, 16, device="meta"))
+
+
 def test_cpu_decoding_on_pages_is_the_contiguous_one(cpu_model):
     """The CPU path gathers the pages and computes what the contiguous cache computes: the same bits."""
     m = cpu_model
