@@ -31,6 +31,10 @@
 // histogram per pass), which no input makes longer than 6 passes.
 //
 // Few rows: a row is cut into parts, one CTA each, and a second launch joins their sums and lists.
+//
+// Times in this file are per call of back-to-back graph replays, where the next launch fills the SMs that a launch's
+// last CTAs leave.  A call alone, behind other data in L2, takes 3 to 7 us more: 1024 bf16 rows of 152064 logits 51 us
+// (93 % of the copy bandwidth) and 56 (85 %), 600 f32 rows 59 and 64, 509 rows with 20 alternatives 36 and 43.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -436,9 +440,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprob_part_kernel(const __gri
 #pragma unroll
     for (int u = 0; u < kLpRuns; ++u) b[u].add(fast);
   };
-  // The next step's pieces are in flight while one's are added; then the steps that not every run fills.
-  // (Two steps per turn save the copies between the buffers but spill a little: 36 us against 39 for 509 rows
-  // with alternatives, 55 against 52 for 1024 without.)
+  // The next step's pieces are in flight while one's are added, two steps per turn so that the buffers change roles
+  // instead of being copied; then the steps that not every run fills.
   static_assert(kLpRuns == 4, "step()");
   uint4 next[kLpRuns];
   const auto load_full = [&](uint4 (&v)[kLpRuns], int base) {
@@ -447,20 +450,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprob_part_kernel(const __gri
   };
   const int full = pieces - (kLpRuns - 1) * runs;  // pieces of the last run, the shortest
   int base = 0;
-  if (TOP) {
-    for (; base + 3 * kLpThreads <= full; base += 2 * kLpThreads) {
-      load_full(next, base + kLpThreads);
-      step(w, base);
-      load_full(w, base + 2 * kLpThreads);
-      step(next, base + kLpThreads);
-    }
-  } else {
-    for (; base + 2 * kLpThreads <= full; base += kLpThreads) {
-      load_full(next, base + kLpThreads);
-      step(w, base);
-#pragma unroll
-      for (int u = 0; u < kLpRuns; ++u) w[u] = next[u];
-    }
+  for (; base + 3 * kLpThreads <= full; base += 2 * kLpThreads) {
+    load_full(next, base + kLpThreads);
+    step(w, base);
+    load_full(w, base + 2 * kLpThreads);
+    step(next, base + kLpThreads);
   }
   for (; base < runs; base += kLpThreads) {
     load(next, base + kLpThreads);
@@ -590,13 +584,13 @@ __global__ void __launch_bounds__(kLpThreads) logprob_join_kernel(const __grid_c
   }
 }
 
-// Parts per row.  Fewer than three rows per SM are cut so that every SM has four CTAs (300 f32 rows: one part
-// 54 us, two 48), into parts of at least 4096 logits, no more than the join's list holds and its threads
-// read.  From there on a row is one CTA (509 rows with 20 alternatives: one part 42 us, two 45, five 49: what a
-// part and the join cost besides the logits), except that without alternatives, where the join is cheap, rows
-// up to six per SM are cut into up to four parts of at least 32768 logits: whole rows, four to an SM, leave most
-// SMs idle at the end (760 rows of 152064 bf16 logits: one part 57 us, four 53; 600 f32 rows 82 and 70; at
-// 1024 rows 64 and 65, and 600 rows of 32000 logits 16 and 20).
+// Parts per row.  Fewer than three rows per SM are cut so that every SM has four CTAs (300 bf16 rows of 152064
+// logits: one part 28.8 us, two 24.3, four 22.5), into parts of at least 4096 logits, no more than the join's list
+// holds and its threads read.  From there on a row is one CTA (509 rows with 20 alternatives: one part 36 us, two 42,
+// four 48: what a part and the join cost besides the logits), except that without alternatives, where the join is
+// cheap, rows up to six per SM are cut into up to four parts of at least 32768 logits: whole rows, four to an SM, leave
+// most SMs idle at the end (600 f32 rows of 152064: one part 68 us, four 59; 760 bf16 rows 44 and 45; at 1024 rows 51
+// and 57, and 600 rows of 32000 logits 12 and 15).
 static void lp_parts(int rows, int V, int top, int n_sm, LpPlan& plan) {
   plan.cap = top > 0 ? top + 32 : 0;
   const int sms = std::max(n_sm, 1);

@@ -28,7 +28,7 @@ namespace skinny {
 __device__ uint32_t g_paged_err;  // error bits of this device's paged calls
 
 constexpr int kPaThreads = 128;
-constexpr int kPaAhead = 2;      // pieces per thread whose loads are issued together (1: 41.4 us for 8191 tokens, 2: 39.4, 4: 42.5)
+constexpr int kPaAhead = 2;      // pieces per thread whose loads are issued together (1: 41.4 us for 8191 tokens, 2: 39.4, 4: 42.5; back-to-back graph replays)
 constexpr int kPaMaxHalf = 128;  // rotation pairs (head dim <= 256)
 
 __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {

@@ -44,6 +44,8 @@
 // lengths are read on the device and the launch does not depend on them (a captured graph serves
 // any).  A CTA whose piece covers an item writes its output; the others write (max, sum, O) to the
 // workspace and the join launch adds them in order, so results do not depend on timing.
+//
+// Times in this file are per call (both launches) of back-to-back graph replays over inputs larger than L2.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -692,7 +694,9 @@ __global__ void __launch_bounds__(kPtThreads, PtShape<D, NB, F8>::kCtas)
       }
     }
     ++seg;
-    if (*static_cast<volatile int*>(&gave_up)) break;  // the results are void; the error word says so
+    // A wait ran out: the results are void, the error word says so.  (The same for every thread: only waits write it,
+    // and the next ones lie behind a barrier that all threads reach after this line.)
+    if (*static_cast<volatile int*>(&gave_up)) break;
   }
   if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicOr(p.seq.err, kErrBitBadInput);
 }
