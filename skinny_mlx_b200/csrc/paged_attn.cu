@@ -64,7 +64,7 @@ namespace skinny {
 
 constexpr int kPtThreads = 128;
 constexpr int kPtWarps = kPtThreads / 32;
-constexpr int kPtLead = 4;             // (0 to 8 tried: verify 31.6 us at 0, 26.2 at 4 and 6, 26.7 at 8; the others hardly move)
+constexpr int kPtLead = 4;             // (0 to 8 tried: verify 31.6 us at 0, 26 at 4 and 6, 26.7 at 8; the others hardly move)
 __device__ __forceinline__ uint32_t pt_transpose(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -874,11 +874,11 @@ PtChoice pt_choose(int T, int Hq, int Hkv) {
 }
 
 // More than 32 rows of bf16 pages (16 of heads of 256) go to the tensor-memory kernel, where its copies can be whole
-// rows of 8 keys (`eights`): 128 rows of 16 K contexts 49 us against 104, 64 rows of 4 K contexts 28 against 42, 40
-// rows 27 against 39, 64 rows of one context of 2 K 16 against 18; heads of 256, 4 K contexts: 64 rows 46 against 97,
-// 20 rows 39 against 56.  With fewer the warps' matrix instructions do as well and begin sooner (32 rows of 8
-// sequences of 4 K: 25 us against 27; heads of 256, 10 rows: 36 against 38), and copies of single keys would take the
-// other longer (32 rows, pages of 7: 315 us against 117).
+// rows of 8 keys (`eights`): 128 rows of 16 K contexts 48 us against 104, 64 rows of 4 K contexts 28 against 41, 40
+// rows 27 against 38, 64 rows of one context of 2 K 16 against 18; heads of 256, 4 K contexts: 64 rows 46 against 97,
+// 20 rows 40 against 56.  With fewer the warps' matrix instructions do as well and begin sooner (32 rows of 8
+// sequences of 4 K: 27.5 us against 27, a call alone 33 against 39; heads of 256, 16 rows: 39 against 42), and copies
+// of single keys would take the other longer (32 rows, pages of 7: 315 us against 117).
 PtChoice pt_choose(int T, int Hq, int Hkv, int D, bool f8, bool eights) {
   const int rows = T * (Hq / Hkv);
   if (!f8 && eights && rows > (D == 256 ? 16 : 32)) {

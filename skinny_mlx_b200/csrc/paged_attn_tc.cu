@@ -9,9 +9,9 @@
 // lanes, each of which exponentiates half of a tile's keys and multiplies zeros for the others: every warp has
 // the same work, and the halves' O are joined at the item's end.  The matrix unit then repeats itself, which
 // costs nothing: a tile of 128 keys takes it some 1600 clocks, the memory 2700 (64 KB at 1/148 of the copy
-// bandwidth).  Measured per call of back-to-back graph replays: two sequences of 100 K and 64 rows 78 us (80 % of the copy bandwidth), four of 16 K
-// and 128 rows 49 us (exponentials and the row maximum, some 2000 clocks a tile in one warp per scheduler; a
-// CTA's beginning and end, some 10 us, weigh on shorter ones: eight of 4 K and 64 rows 28 us).
+// bandwidth).  Measured per call of back-to-back graph replays: two sequences of 100 K and 64 rows 79 us (79 % of the
+// copy bandwidth), four of 16 K and 128 rows 48 us (exponentials and the row maximum, some 2000 clocks a tile in one
+// warp per scheduler; a CTA's beginning and end, some 10 us, weigh on shorter ones: eight of 4 K and 64 rows 28 us).
 //
 // Seven warps: four of softmax, one that issues the matrix instructions, one that copies keys, one values.
 // S(n + 2) follows O += P(n) V(n), while the softmax works on S(n + 1).  The maximum of a row is renewed only when a
