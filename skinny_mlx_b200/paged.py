@@ -288,8 +288,8 @@ class PageTable:
 
 def device_errors(device: torch.device | None = None, clear: bool = False) -> int:
     """The error bits of the paged calls made on `device` so far (synchronises with the current stream; calls on
-    other streams are to be waited for first): 0; bit 9: a sequence or page id out of range; bit 0: a bounded wait ran out, the outputs of that call are
-    void (skinny_b200.h).  clear: reset them afterwards."""
+    other streams are to be waited for first): 0; bit 9: a sequence or page id out of range; bit 0: a bounded
+    wait ran out, the outputs of that call are void (skinny_b200.h).  clear: reset them afterwards."""
     word = ctypes.c_uint32()
     with torch.cuda.device(device):
         stream = torch.cuda.current_stream()

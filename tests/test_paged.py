@@ -871,3 +871,28 @@ def test_pools_of_nothing_are_refused(cuda_lib, dev):
         paged.attention(c.q, *none, c.table, c.lengths)
     with pytest.raises(ValueError):
         paged.append(None, c.k[:, :, :0], c.v[:, :, :0], *none, c.table, c.lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hq,T", [(64, 1, 1), (128, 4, 1), (256, 2, 4), (128, 4, 5)])
+def test_every_e4m3_number_as_key_and_value(cuda_lib, dev, D, Hq, T):
+    """Each of the 256 codes is one sequence's only visible key and value: the output is the value itself, exactly (with
+    a scale of 1 all of them are bf16 numbers), the log-sum-exp its product with the query."""
+    codes = torch.arange(256, dtype=torch.uint8, device=dev).view(F8)
+    c = Case(dev, [0] * 256, T=T, Hq=Hq, Hkv=1, D=D, page=8, kv=F8, seed=1)
+    c.scales = {"k_scale": torch.full((1,), 0.5, device=dev), "v_scale": torch.ones(1, device=dev)}
+    c.kp.view(torch.uint8).zero_()
+    for t in range(T):
+        slot = c.table[:, t // 8].long()
+        c.kp.view(torch.uint8)[slot, 0, t % 8, 3] = codes.view(torch.uint8)
+        c.vp.view(torch.uint8)[slot, 0, t % 8] = codes.view(torch.uint8)[:, None]
+    c.q = torch.zeros_like(c.q)
+    c.q[..., 3] = 2
+    o, lse = c.attend(scale=1.0, window=1)
+    want = codes.float()
+    assert want.isnan().sum() == 2
+    ok = ~want.isnan()
+    assert torch.equal(o.float()[ok], want[ok][:, None, None, None].expand(-1, T, Hq, D))
+    assert o[~ok].isnan().all()
+    # (the score goes to powers of two and back, and log2 of the sum, which is 1, is 0: three roundings)
+    assert torch.allclose(lse[ok], want[ok][:, None, None].expand(-1, T, Hq), rtol=2.0 ** -21, atol=2.0 ** -21)
